@@ -60,6 +60,7 @@ extern "C" {
 
 #define MXG_DTYPE_BF16 0
 #define MXG_DTYPE_F32 1
+#define MXG_DTYPE_F16 2 /* router logits only */
 
 #define MXG_MAX_GROUPS 256
 
@@ -252,6 +253,27 @@ MXG_API int mxg_ep_regroup(const int32_t* recv_counts, int world, int e_local, i
 MXG_API int mxg_ep_combine(const void* rows, const int32_t* slot_pos, const float* weights,
                            int64_t n_tokens, int topk, int64_t hidden, void* out, void* stream);
 
+/* mxg_ep_combine over n_rows rows: a position >= n_rows is skipped and sets the
+ * device error word to MXG_ERR_INVALID_ARGUMENT. */
+MXG_API int mxg_ep_combine_rows(const void* rows, int64_t n_rows, const int32_t* slot_pos,
+                                const float* weights, int64_t n_tokens, int topk, int64_t hidden,
+                                void* out, void* stream);
+
+/* Gradient of mxg_ep_combine: from dout [n_tokens, hidden] bf16 and the n_rows
+ * rows that were combined (send order),
+ *   drows[slot_pos[t*topk+j]] = w[t*topk+j] * dout[t]            (bf16),
+ *   dweights[t*topk+j]        = <dout[t], rows[slot_pos[t*topk+j]]>  (fp32).
+ * Either output may be null (rows may be null without dweights; null weights =
+ * 1).  A negative position has no row: its dweights are 0.  One that is >=
+ * n_rows is skipped too and sets the device error word to
+ * MXG_ERR_INVALID_ARGUMENT.  slot_pos names a position at most once, as
+ * mxg_ep_route gives it.  Rows of drows that it does not name become zero with
+ * seen (n_rows bytes of workspace), and are left as they were when it is null. */
+MXG_API int mxg_ep_combine_bwd(const void* dout, const void* rows, const int32_t* slot_pos,
+                               const float* weights, int64_t n_tokens, int topk, int64_t hidden,
+                               int64_t n_rows, void* drows, float* dweights, uint8_t* seen,
+                               void* stream);
+
 /* h = silu(g) * u for gu rows [g (inter) | u (inter)], bf16 (the gate/up ->
  * down activation of the expert FFN, e2e_bench.py:56-61). */
 MXG_API int mxg_swiglu(const void* gu, int64_t rows, int64_t inter, void* h, void* stream);
@@ -260,6 +282,101 @@ MXG_API int mxg_swiglu(const void* gu, int64_t rows, int64_t inter, void* h, voi
  * dh (bf16 [rows, inter]). */
 MXG_API int mxg_swiglu_bwd(const void* gu, const void* dh, int64_t rows, int64_t inter, void* dgu,
                            void* stream);
+
+/* ---- router: each token's experts and their weights ----
+ * The gate in front of mxg_ep_route (the reference takes it from torchtitan's
+ * router, port_mxfp8.py:74).  logits [n_tokens, num_experts] (bf16, f16 or
+ * f32, row stride ld elements), s = softmax or sigmoid of a row, choice =
+ * s + bias (bias f32 [num_experts] or null; it takes part in the choice only):
+ *   - experts in `groups` equal groups of consecutive ones; a group counts by
+ *     its best choice (MXG_GROUP_MAX) or the sum of its two best
+ *     (MXG_GROUP_TOP2); the topk_groups best groups stay, ties to the lowest;
+ *   - ids = the topk largest choices among them, descending, ties to the
+ *     lowest index.  The order is that of the scores in 64 bits; without a
+ *     bias it is the logits' (the scores rise with them).  A NaN is ordered as
+ *     -inf;
+ *   - weights = scale * s[ids], divided by the sum of the s[ids] first when
+ *     renormalize is set (f32; scale > 0).  A logit of -inf has weight 0, also
+ *     where nothing else is left; a softmax row with a NaN or +inf has NaN
+ *     weights (and ids in range).
+ * num_experts <= MXG_EP_MAX_EXPERTS, topk <= MXG_ROUTER_MAX_TOPK, groups <=
+ * MXG_ROUTER_MAX_GROUPS. */
+#define MXG_SCORE_SOFTMAX 0
+#define MXG_SCORE_SIGMOID 1
+#define MXG_GROUP_MAX 0
+#define MXG_GROUP_TOP2 1
+#define MXG_ROUTER_MAX_TOPK 32
+#define MXG_ROUTER_MAX_GROUPS 32
+MXG_API int mxg_router_topk(const void* logits, int64_t ld, int dtype, int64_t n_tokens,
+                            int num_experts, int topk, int score, const float* bias, int groups,
+                            int topk_groups, int group_score, int renormalize, float scale,
+                            float* weights, int32_t* ids, void* stream);
+
+/* Gradient of the logits (same dtype, row stride ld_out; every element is
+ * written) from dweights [n_tokens, topk], and the weights and ids that
+ * mxg_router_topk gave.  The choice itself has no gradient.  An id out of
+ * range is skipped and sets the device error word; one named twice gets the
+ * sum. */
+MXG_API int mxg_router_topk_bwd(const void* logits, int64_t ld, int dtype, int64_t n_tokens,
+                                int num_experts, int topk, int score, int renormalize, float scale,
+                                const float* weights, const int32_t* ids, const float* dweights,
+                                void* dlogits, int64_t ld_out, void* stream);
+
+/* ---- AdamW over many tensors in one launch ----
+ * Moments are flat arrays in which tensor i starts at element offset[i], a
+ * multiple of MXG_ADAMW_BLOCK; gaps hold zeros.  With g the gradient, t the
+ * step (counted from 1) and every operation in f32:
+ *   m = b1 m + (1-b1) g,  v = b2 v + (1-b2) g^2,
+ *   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps).
+ * state_bits 32: moments are f32.  state_bits 8: a byte a value and an f32
+ * scale a block of 256 values, the block's largest (at least 2^-100).  The
+ * first moment's byte is a sign, 4 exponent and 3 mantissa bits, the second's 5
+ * exponent and 3 mantissa bits, of the value relative to the scale (1.0 is
+ * 0x78 and 0xF8), without codes for infinity; they are rounded stochastically
+ * by bits hashed from (seed, step, element), so an average moves by less than
+ * a code's step without bias.  A second moment above zero never becomes 0.
+ * Weights are f32, or bf16 with an f32 copy (master) that is updated and then
+ * rounded to nearest, or bf16 without one, rounded stochastically (to nearest
+ * would lose every update under half a step). */
+#define MXG_ADAMW_BLOCK 256
+#define MXG_ADAMW_CHUNK 4096      /* elements a table entry covers */
+#define MXG_ADAMW_F32 0           /* kinds of weights */
+#define MXG_ADAMW_BF16_MASTER 1
+#define MXG_ADAMW_BF16 2
+typedef struct mxg_adamw_tensor {
+  void* param;
+  int64_t numel;
+  int64_t offset;                 /* first element in the moments            */
+  int64_t master;                 /* first element in the f32 copies, or -1  */
+  float weight_decay;
+  int32_t kind;                   /* MXG_ADAMW_*                              */
+  int64_t first_chunk;            /* first entry of this tensor in `chunks`  */
+} mxg_adamw_tensor;
+
+/* tensors [n_tensors] and chunks [n_chunks] are device arrays: chunks holds,
+ * tensor after tensor, its index once for each MXG_ADAMW_CHUNK of its elements
+ * (rounded up).  grads [n_tensors] is a HOST array of device addresses (0: no
+ * gradient, the tensor and its moments are left as they are) and grad_dtypes
+ * [n_tensors] the MXG_DTYPE_ of each (bf16 or f32); chunk_begin [n_tensors + 1]
+ * a HOST array, the first entry of each tensor.  scales are [elements / 256]
+ * f32, null with 32 bits; master may be null without such tensors.  step is one
+ * int64 on the device, the steps taken so far: it is read and then raised by
+ * one, so a captured launch counts on when it is replayed.  lr_ptr, when not
+ * null, is one f32 on the device that replaces lr.  done is one int32 on the
+ * device, zero between calls.  Calls on the same moments run one after the
+ * other. */
+MXG_API int mxg_adamw_step(const mxg_adamw_tensor* tensors, int n_tensors, const int32_t* chunks,
+                           const int64_t* chunk_begin, const uint64_t* grads,
+                           const int32_t* grad_dtypes, int state_bits, void* exp_avg,
+                           void* exp_avg_sq, float* exp_avg_scale, float* exp_avg_sq_scale,
+                           float* master, int64_t* step, int32_t* done, double lr,
+                           const float* lr_ptr, double beta1, double beta2, double eps,
+                           uint64_t seed, void* stream);
+
+/* The f32 values of 8-bit moments (n elements, a multiple of 256). */
+MXG_API int mxg_adamw_moments(const void* exp_avg, const void* exp_avg_sq, const float* exp_avg_scale,
+                              const float* exp_avg_sq_scale, int64_t n, float* exp_avg_out,
+                              float* exp_avg_sq_out, void* stream);
 
 /* ---- expert parallelism over NVLink peer memory ----
  * Receive buffers are shared between the ranks of one node with CUDA IPC; a

@@ -5,6 +5,7 @@ functions below raise; there is no CPU or library fallback.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import re
@@ -27,10 +28,17 @@ MXG_ERR_BAD_OFFSETS = 7
 MXG_ERR_UNSUPPORTED_DEVICE = 8
 MXG_ERR_TOO_MANY_GROUPS = 9
 OFFS_LEADING_ZERO, OFFS_CUMULATIVE, OFFS_SIZES, OFFS_AUTO = 0, 1, 2, 3
-DTYPE_BF16, DTYPE_F32 = 0, 1
+DTYPE_BF16, DTYPE_F32, DTYPE_F16 = 0, 1, 2
 MAX_GROUPS = 256
+EP_MAX_EXPERTS = 384
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+GROUP_MAX, GROUP_TOP2 = 0, 1
+ROUTER_MAX_TOPK, ROUTER_MAX_GROUPS = 32, 32
+ADAMW_BLOCK, ADAMW_CHUNK = 256, 4096
+ADAMW_F32, ADAMW_BF16_MASTER, ADAMW_BF16 = 0, 1, 2
 
 _c_i64, _c_int, _c_size, _vp = ctypes.c_int64, ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p
+_c_f32, _c_f64, _c_u64 = ctypes.c_float, ctypes.c_double, ctypes.c_uint64
 _i32p = ctypes.POINTER(ctypes.c_int32)
 
 _PROTOS = {
@@ -65,6 +73,15 @@ _PROTOS = {
     "mxg_gather_rows": (_c_int, [_vp, _c_i64, _c_i64, _vp, _c_i64, _vp, _vp]),
     "mxg_ep_regroup": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp]),
     "mxg_ep_combine": (_c_int, [_vp, _vp, _vp, _c_i64, _c_int, _c_i64, _vp, _vp]),
+    "mxg_ep_combine_rows": (_c_int, [_vp, _c_i64, _vp, _vp, _c_i64, _c_int, _c_i64, _vp, _vp]),
+    "mxg_ep_combine_bwd": (_c_int, [_vp, _vp, _vp, _vp, _c_i64, _c_int, _c_i64, _c_i64, _vp, _vp, _vp, _vp]),
+    "mxg_router_topk": (_c_int, [_vp, _c_i64, _c_int, _c_i64, _c_int, _c_int, _c_int, _vp, _c_int, _c_int,
+                                 _c_int, _c_int, _c_f32, _vp, _vp, _vp]),
+    "mxg_router_topk_bwd": (_c_int, [_vp, _c_i64, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_f32, _vp,
+                                     _vp, _vp, _vp, _c_i64, _vp]),
+    "mxg_adamw_step": (_c_int, [_vp, _c_int, _vp, _vp, _vp, _vp, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_f64,
+                                _vp, _c_f64, _c_f64, _c_f64, _c_u64, _vp]),
+    "mxg_adamw_moments": (_c_int, [_vp, _vp, _vp, _vp, _c_i64, _vp, _vp, _vp]),
     "mxg_swiglu": (_c_int, [_vp, _c_i64, _c_i64, _vp, _vp]),
     "mxg_swiglu_bwd": (_c_int, [_vp, _vp, _c_i64, _c_i64, _vp, _vp]),
     "mxg_peer_alloc": (_c_int, [_c_size, ctypes.POINTER(_vp), _vp]),
@@ -152,6 +169,15 @@ def raise_device_error() -> None:
 
 def stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is the current one: the C ABI launches on
+    the current device, and a tensor may lie on another."""
+    return _SAME_DEVICE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def ptr(t) -> int | None:

@@ -61,3 +61,53 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, offs: torch.Tensor,
                out_dtype=torch.bfloat16) -> torch.Tensor:
     """y = x @ W[g]^T over the row groups of x, MXFP8 forward and backward."""
     return _GroupedMM.apply(x, w, offs, out_dtype)
+
+
+class _RouterTopk(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, topk, score, bias, groups, topk_groups, group_score, renormalize, scale):
+        weights, ids = ops.router_topk(logits, topk, score=score, bias=bias, groups=groups, topk_groups=topk_groups,
+                                       group_score=group_score, renormalize=renormalize, scale=scale)
+        ctx.how = dict(score=score, renormalize=renormalize, scale=scale)
+        ctx.save_for_backward(logits, weights, ids)
+        ctx.mark_non_differentiable(ids)
+        return weights, ids
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dweights, _):
+        logits, weights, ids = ctx.saved_tensors
+        return (ops.router_topk_bwd(logits, weights, ids, dweights, **ctx.how),) + (None,) * 8
+
+
+def router_topk(logits: torch.Tensor, topk: int, *, score: str = "softmax", bias=None, groups: int = 1,
+                topk_groups: int | None = None, group_score: str = "max", renormalize: bool = True,
+                scale: float = 1.0):
+    """``ops.router_topk`` with a gradient: (weights [n, topk] fp32, ids [n, topk]
+    int32) of logits [n, E]; the weights' gradient flows to the logits, the
+    choice (ids, bias, groups) has none."""
+    return _RouterTopk.apply(logits, topk, score, bias, groups, topk_groups, group_score, renormalize, scale)
+
+
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, slot_pos, weights):
+        out = ops.combine(rows, slot_pos, weights)
+        ctx.save_for_backward(rows, slot_pos, weights)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        rows, slot_pos, weights = ctx.saved_tensors
+        drows, dweights = ops.combine_bwd(dout.to(torch.bfloat16), rows, slot_pos, weights,
+                                          need_rows=ctx.needs_input_grad[0],
+                                          need_weights=weights is not None and ctx.needs_input_grad[2])
+        return drows, None, dweights if dweights is None else dweights.to(weights.dtype)
+
+
+def combine(rows: torch.Tensor, slot_pos: torch.Tensor, weights: torch.Tensor | None = None) -> torch.Tensor:
+    """out[t] = sum_j weights[t, j] * rows[slot_pos[t, j]] (rows bf16 [P, H] in
+    send order, slot_pos int32 [n, topk] as ``CudaEpOps.route`` gives it, None
+    weights = 1), with gradients for the rows and the weights."""
+    return _Combine.apply(rows, slot_pos, weights)

@@ -11,6 +11,8 @@
 //             local expert) -> expert-major groups padded to `pad` rows, and
 //             the inverse map used to send results back.
 //   combine:  out[t] = sum_j w[t, j] * rows[inv[t * k + j]] (fp32 sum, bf16 out).
+//   combine's gradient: drows[inv[t * k + j]] = w[t, j] * dout[t] and
+//             dw[t, j] = <dout[t], rows[inv[t * k + j]]>.
 //   swiglu:   h = silu(g) * u for gu = [g | u] rows (bf16 in/out), and its
 //             backward dgu = [dg | du] from dh.
 #include <cuda_bf16.h>
@@ -192,14 +194,18 @@ __global__ void regroup_kernel(const int32_t* __restrict__ recv_counts, int worl
 __global__ void __launch_bounds__(128) combine_kernel(const __nv_bfloat16* __restrict__ rows,
                                                       const int32_t* __restrict__ inv,
                                                       const float* __restrict__ w, int topk,
-                                                      int64_t hidden,
-                                                      __nv_bfloat16* __restrict__ out) {
+                                                      int64_t hidden, int64_t n_rows,
+                                                      __nv_bfloat16* __restrict__ out, int* err) {
   const int64_t t = blockIdx.x;
   for (int64_t c = int64_t(threadIdx.x) * 8; c < hidden; c += int64_t(blockDim.x) * 8) {
     float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     for (int j = 0; j < topk; ++j) {
       const int32_t p = inv[t * topk + j];
       if (p < 0) continue;
+      if (p >= n_rows) {
+        if (c == 0) atomicCAS(err, 0, MXG_ERR_INVALID_ARGUMENT);
+        continue;
+      }
       const float wj = w ? w[t * topk + j] : 1.0f;
       const uint4 v = __ldg(reinterpret_cast<const uint4*>(rows + int64_t(p) * hidden + c));
       const __nv_bfloat162* h2 = reinterpret_cast<const __nv_bfloat162*>(&v);
@@ -215,6 +221,98 @@ __global__ void __launch_bounds__(128) combine_kernel(const __nv_bfloat16* __res
 #pragma unroll
     for (int q = 0; q < 4; ++q) o2[q] = __floats2bfloat162_rn(acc[2 * q], acc[2 * q + 1]);
     *reinterpret_cast<uint4*>(out + t * hidden + c) = o;
+  }
+}
+
+// Gradient of combine.  One block a token: its dout row stays in registers
+// (U vectors of 8 a thread) while the token's k rows pass by once, each giving
+// a partial dot product and taking the row's gradient.  Bound by HBM (k rows
+// in, k rows out, one dout row).  The dot products are summed in a fixed
+// order: over a thread's columns, over the warp, over the warps.
+template <int U>
+__global__ void __launch_bounds__(256) combine_bwd_kernel(const __nv_bfloat16* __restrict__ dout,
+                                                          const __nv_bfloat16* __restrict__ rows,
+                                                          const int32_t* __restrict__ inv,
+                                                          const float* __restrict__ w, int topk, int64_t hidden,
+                                                          int64_t n_rows, __nv_bfloat16* __restrict__ drows,
+                                                          float* __restrict__ dw, uint8_t* __restrict__ seen,
+                                                          int* err) {
+  extern __shared__ float part[];  // [topk][warps]
+  const int64_t t = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int64_t vecs = hidden / 8;
+  for (int64_t c0 = 0; c0 < vecs; c0 += int64_t(U) * blockDim.x) {
+    uint4 d[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t c = c0 + u * int64_t(blockDim.x) + threadIdx.x;
+      d[u] = c < vecs ? __ldg(reinterpret_cast<const uint4*>(dout + t * hidden) + c) : make_uint4(0, 0, 0, 0);
+    }
+    for (int j = 0; j < topk; ++j) {
+      const int64_t p = inv[t * topk + j];
+      float dot = 0.0f;
+      if (p >= 0 && p < n_rows) {
+        if (dw) {
+          uint4 x[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int64_t c = c0 + u * int64_t(blockDim.x) + threadIdx.x;
+            x[u] = c < vecs ? __ldcs(reinterpret_cast<const uint4*>(rows + p * hidden) + c) : make_uint4(0, 0, 0, 0);
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const uint32_t* a = reinterpret_cast<const uint32_t*>(&d[u]);
+            const uint32_t* b = reinterpret_cast<const uint32_t*>(&x[u]);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              dot = fmaf(bf16_lo(a[q]), bf16_lo(b[q]), dot);
+              dot = fmaf(bf16_hi(a[q]), bf16_hi(b[q]), dot);
+            }
+          }
+        }
+        if (drows) {
+          if (seen && c0 == 0 && threadIdx.x == 0) seen[p] = 1;
+          const float wj = w ? w[t * topk + j] : 1.0f;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int64_t c = c0 + u * int64_t(blockDim.x) + threadIdx.x;
+            const uint32_t* a = reinterpret_cast<const uint32_t*>(&d[u]);
+            uint4 o;
+            uint32_t* b = reinterpret_cast<uint32_t*>(&o);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) b[q] = pack2_bf16(wj * bf16_lo(a[q]), wj * bf16_hi(a[q]));
+            if (c < vecs) __stcs(reinterpret_cast<uint4*>(drows + p * hidden) + c, o);
+          }
+        }
+      } else if (p >= n_rows && threadIdx.x == 0) {
+        atomicCAS(err, 0, MXG_ERR_INVALID_ARGUMENT);
+      }
+      if (dw) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        if (lane == 0) part[j * warps + warp] = c0 == 0 ? dot : part[j * warps + warp] + dot;
+      }
+    }
+  }
+  if (!dw) return;
+  __syncthreads();
+  for (int j = threadIdx.x; j < topk; j += blockDim.x) {
+    float s = 0.0f;
+    for (int q = 0; q < warps; ++q) s += part[j * warps + q];
+    dw[t * topk + j] = s;
+  }
+}
+
+// Zeros in the rows that combine_bwd_kernel did not write.
+__global__ void __launch_bounds__(256) zero_unseen_rows_kernel(const uint8_t* __restrict__ seen, int64_t n_rows,
+                                                               int64_t vecs, uint4* __restrict__ rows) {
+  for (int64_t r0 = int64_t(blockIdx.x) * 256; r0 < n_rows; r0 += int64_t(gridDim.x) * 256) {
+    const bool zero = r0 + threadIdx.x < n_rows && !seen[r0 + threadIdx.x];
+    if (!__syncthreads_or(zero)) continue;
+    for (int64_t r = r0; r < min(n_rows, r0 + 256); ++r) {
+      if (seen[r]) continue;
+      for (int64_t c = threadIdx.x; c < vecs; c += 256) rows[r * vecs + c] = make_uint4(0, 0, 0, 0);
+    }
   }
 }
 
@@ -350,17 +448,65 @@ extern "C" int mxg_ep_regroup(const int32_t* recv_counts, int world, int e_local
 
 extern "C" int mxg_ep_combine(const void* rows, const int32_t* slot_pos, const float* weights,
                               int64_t n_tokens, int topk, int64_t hidden, void* out, void* stream) {
-  if (n_tokens < 0 || topk < 1 || hidden < 0) return MXG_ERR_INVALID_ARGUMENT;
+  if (n_tokens > 0 && hidden > 0 && !rows) return MXG_ERR_INVALID_ARGUMENT;
+  return mxg_ep_combine_rows(rows, INT64_MAX, slot_pos, weights, n_tokens, topk, hidden, out, stream);
+}
+
+extern "C" int mxg_ep_combine_rows(const void* rows, int64_t n_rows, const int32_t* slot_pos,
+                                   const float* weights, int64_t n_tokens, int topk, int64_t hidden,
+                                   void* out, void* stream) {
+  if (n_tokens < 0 || topk < 1 || hidden < 0 || n_rows < 0) return MXG_ERR_INVALID_ARGUMENT;
   if (hidden % 8 != 0) return MXG_ERR_BAD_SHAPE;
   if (n_tokens == 0 || hidden == 0) return MXG_OK;
-  if (!rows || !slot_pos || !out) return MXG_ERR_INVALID_ARGUMENT;
+  if ((!rows && n_rows > 0) || !slot_pos || !out) return MXG_ERR_INVALID_ARGUMENT;
   if (!aligned16(rows) || !aligned16(out)) return MXG_ERR_MISALIGNED;
   if (n_tokens > INT32_MAX) return MXG_ERR_BAD_SHAPE;
   int st = check_device();
   if (st) return st;
+  int* err = device_error_word();
+  if (!err) return MXG_ERR_CUDA;
   combine_kernel<<<unsigned(n_tokens), 128, 0, (cudaStream_t)stream>>>(
-      reinterpret_cast<const __nv_bfloat16*>(rows), slot_pos, weights, topk, hidden,
-      reinterpret_cast<__nv_bfloat16*>(out));
+      reinterpret_cast<const __nv_bfloat16*>(rows), slot_pos, weights, topk, hidden, n_rows,
+      reinterpret_cast<__nv_bfloat16*>(out), err);
+  return cuda_status(cudaGetLastError());
+}
+
+extern "C" int mxg_ep_combine_bwd(const void* dout, const void* rows, const int32_t* slot_pos, const float* weights,
+                                  int64_t n_tokens, int topk, int64_t hidden, int64_t n_rows, void* drows,
+                                  float* dweights, uint8_t* seen, void* stream) {
+  if (n_tokens < 0 || topk < 1 || hidden < 0 || n_rows < 0) return MXG_ERR_INVALID_ARGUMENT;
+  if (hidden % 8 != 0 || topk > MXG_EP_MAX_EXPERTS || n_tokens > INT32_MAX) return MXG_ERR_BAD_SHAPE;
+  if (!drows && !dweights) return MXG_OK;
+  int st;
+  if (n_tokens == 0 || hidden == 0) {  // no product: zeros
+    if ((st = check_device())) return st;
+    if (dweights && n_tokens &&
+        cudaMemsetAsync(dweights, 0, sizeof(float) * n_tokens * topk, (cudaStream_t)stream) != cudaSuccess)
+      return MXG_ERR_CUDA;
+    if (drows && seen && n_rows && hidden &&
+        cudaMemsetAsync(drows, 0, 2 * n_rows * hidden, (cudaStream_t)stream) != cudaSuccess)
+      return MXG_ERR_CUDA;
+    return MXG_OK;
+  }
+  if (!dout || (!rows && dweights && n_rows > 0) || !slot_pos) return MXG_ERR_INVALID_ARGUMENT;
+  if (!aligned16(dout) || !aligned16(rows) || !aligned16(drows)) return MXG_ERR_MISALIGNED;
+  if ((st = check_device())) return st;
+  int* err = device_error_word();
+  if (!err) return MXG_ERR_CUDA;
+  const int64_t vecs = hidden / 8;
+  const int threads = int(std::min<int64_t>(256, (vecs + 31) / 32 * 32));
+  const size_t smem = sizeof(float) * size_t(topk) * (threads / 32);
+  if (seen && drows && n_rows && cudaMemsetAsync(seen, 0, n_rows, (cudaStream_t)stream) != cudaSuccess)
+    return MXG_ERR_CUDA;
+  auto* kernel = vecs <= 256 ? combine_bwd_kernel<1> : vecs <= 512 ? combine_bwd_kernel<2> : combine_bwd_kernel<4>;
+  kernel<<<unsigned(n_tokens), threads, smem, (cudaStream_t)stream>>>(
+      reinterpret_cast<const __nv_bfloat16*>(dout), reinterpret_cast<const __nv_bfloat16*>(rows), slot_pos, weights,
+      topk, hidden, n_rows, reinterpret_cast<__nv_bfloat16*>(drows), dweights, seen, err);
+  if (seen && drows && n_rows) {
+    const int64_t blocks = std::min<int64_t>((n_rows + 255) / 256, int64_t(num_sms()) * 4);
+    zero_unseen_rows_kernel<<<unsigned(blocks), 256, 0, (cudaStream_t)stream>>>(seen, n_rows, vecs,
+                                                                              reinterpret_cast<uint4*>(drows));
+  }
   return cuda_status(cudaGetLastError());
 }
 

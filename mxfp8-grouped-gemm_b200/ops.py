@@ -11,6 +11,9 @@ from . import _lib
 
 _FP8 = (torch.float8_e4m3fn, torch.uint8)
 _SC = (torch.uint8, getattr(torch, "float8_e8m0fnu", torch.uint8))
+_LOGITS = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16, torch.float32: _lib.DTYPE_F32}
+_SCORES = {"softmax": _lib.SCORE_SOFTMAX, "sigmoid": _lib.SCORE_SIGMOID}
+_GROUP_SCORES = {"max": _lib.GROUP_MAX, "top2": _lib.GROUP_TOP2}
 _OUT = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
 
 
@@ -283,6 +286,167 @@ def swiglu_bwd(gu: torch.Tensor, dh: torch.Tensor) -> torch.Tensor:
                                           dgu.data_ptr(), _lib.stream_ptr(gu.device)),
                "mxg_swiglu_bwd")
     return dgu
+
+
+# ---------------------------------------------------------------- router
+def _logits(logits, name="logits"):
+    """(tensor whose rows are contiguous, row stride)"""
+    if logits.dtype not in _LOGITS or logits.dim() != 2:
+        raise TypeError(f"{name} must be a 2-D bf16, fp16 or fp32 tensor")
+    n, E = logits.shape
+    if not 1 <= E <= _lib.EP_MAX_EXPERTS:
+        raise ValueError(f"{name} has {E} experts, 1 to {_lib.EP_MAX_EXPERTS} are supported")
+    _cuda(logits, name)
+    if logits.stride(1) != 1 or logits.stride(0) < E:
+        logits = logits.contiguous()
+    return logits, logits.stride(0)
+
+
+def _per_choice(t, name, dtype, like):
+    if t.shape != like:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(like)}")
+    _cuda(t, name)
+    if t.dtype != dtype:
+        t = t.to(dtype)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _score(score, scale):
+    if score not in _SCORES:
+        raise ValueError(f"score must be 'softmax' or 'sigmoid', got {score!r}")
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    return _SCORES[score]
+
+
+def router_topk(logits: torch.Tensor, topk: int, *, score: str = "softmax", bias=None, groups: int = 1,
+                topk_groups: int | None = None, group_score: str = "max", renormalize: bool = True,
+                scale: float = 1.0):
+    """Experts of every token and their weights: logits [n, E] (bf16, fp16 or
+    fp32; rows may be strided) -> (weights [n, topk] fp32, ids [n, topk] int32).
+
+    s = softmax or sigmoid of a token's logits.  The topk experts with the
+    largest s + bias are taken (bias [E], e.g. for balance, takes part in the
+    choice only), in descending order, ties to the lowest index.  With
+    ``groups`` > 1 they come from the ``topk_groups`` best groups of E/groups
+    consecutive experts; a group counts by its best expert ("max") or the sum
+    of its two best ("top2").  weights = scale * s of the chosen, divided by
+    their sum first when ``renormalize``.  An expert whose logit is -inf has
+    weight 0, also in a row where nothing is left; a softmax row with a NaN
+    or +inf has NaN weights.  ``ExpertParallel.dispatch`` takes the ids and
+    ``combine`` the weights.  The differentiable form is
+    ``autograd.router_topk``."""
+    code = _score(score, scale)
+    if group_score not in _GROUP_SCORES:
+        raise ValueError(f"group_score must be 'max' or 'top2', got {group_score!r}")
+    if topk_groups is None:
+        topk_groups = groups
+    logits, ld = _logits(logits)
+    n, E = logits.shape
+    if not 1 <= groups <= _lib.ROUTER_MAX_GROUPS or E % groups or not 1 <= topk_groups <= groups:
+        raise ValueError(f"groups={groups} (at most {_lib.ROUTER_MAX_GROUPS}) must divide {E} experts and "
+                         f"topk_groups={topk_groups} lie in 1..groups")
+    if not 1 <= topk <= min(_lib.ROUTER_MAX_TOPK, topk_groups * (E // groups)):
+        raise ValueError(f"topk={topk} must lie in 1..{min(_lib.ROUTER_MAX_TOPK, topk_groups * (E // groups))}")
+    dev = logits.device
+    if bias is not None:
+        bias = _per_choice(bias, "bias", torch.float32, (E,))
+        if bias.device != dev:
+            raise ValueError("bias and logits must be on one device")
+    weights = torch.empty(n, topk, dtype=torch.float32, device=dev)
+    ids = torch.empty(n, topk, dtype=torch.int32, device=dev)
+    with _lib.on_device(dev):
+        _lib.check(_lib.load().mxg_router_topk(
+            logits.data_ptr(), ld, _LOGITS[logits.dtype], n, E, topk, code, _lib.ptr(bias), groups, topk_groups,
+            _GROUP_SCORES[group_score], renormalize, scale, weights.data_ptr(), ids.data_ptr(),
+            _lib.stream_ptr(dev)), "mxg_router_topk")
+    return weights, ids
+
+
+def router_topk_bwd(logits: torch.Tensor, weights: torch.Tensor, ids: torch.Tensor, dweights: torch.Tensor, *,
+                    score: str = "softmax", renormalize: bool = True, scale: float = 1.0) -> torch.Tensor:
+    """Gradient of the logits [n, E] (their dtype) from that of the weights
+    [n, topk], given the ``weights`` and ``ids`` of ``router_topk`` with the
+    same score, renormalize and scale.  The choice has no gradient (nor has a
+    bias or the grouping).  An id out of range is skipped and sets the device
+    error word; an id named twice in a row gets the sum."""
+    code = _score(score, scale)
+    logits, ld = _logits(logits)
+    n, E = logits.shape
+    if weights.dim() != 2 or weights.shape[0] != n or not 1 <= weights.shape[1] <= min(E, _lib.ROUTER_MAX_TOPK):
+        raise ValueError(f"weights has shape {tuple(weights.shape)}, expected ({n}, topk)")
+    if ids.dtype != torch.int32:
+        raise TypeError(f"ids must be int32, got {ids.dtype}")
+    shape, dev = weights.shape, logits.device
+    weights = _per_choice(weights, "weights", torch.float32, shape)
+    ids = _per_choice(ids, "ids", torch.int32, shape)
+    dweights = _per_choice(dweights, "dweights", torch.float32, shape)
+    if not weights.device == ids.device == dweights.device == dev:
+        raise ValueError("logits, weights, ids and dweights must be on one device")
+    out = torch.empty(n, E, dtype=logits.dtype, device=dev)
+    with _lib.on_device(dev):
+        _lib.check(_lib.load().mxg_router_topk_bwd(
+            logits.data_ptr(), ld, _LOGITS[logits.dtype], n, E, shape[1], code, renormalize, scale,
+            weights.data_ptr(), ids.data_ptr(), dweights.data_ptr(), out.data_ptr(), E, _lib.stream_ptr(dev)),
+            "mxg_router_topk_bwd")
+    return out
+
+
+# ---------------------------------------------------------------- combine
+def _combine_args(rows, slot_pos, weights):
+    if rows.dtype != torch.bfloat16 or rows.dim() != 2 or rows.shape[1] % 8:
+        raise TypeError("rows must be a 2-D bf16 tensor with a multiple of 8 columns")
+    if slot_pos.dtype != torch.int32 or slot_pos.dim() != 2 or not 1 <= slot_pos.shape[1] <= _lib.EP_MAX_EXPERTS:
+        raise TypeError(f"slot_pos must be an int32 [n, topk] tensor, topk at most {_lib.EP_MAX_EXPERTS}")
+    _cuda(rows, "rows")
+    _cuda(slot_pos, "slot_pos")
+    if weights is not None:
+        weights = _per_choice(weights, "weights", torch.float32, slot_pos.shape)
+    if slot_pos.device != rows.device or (weights is not None and weights.device != rows.device):
+        raise ValueError("rows, slot_pos and weights must be on one device")
+    return rows.contiguous(), slot_pos.contiguous(), weights
+
+
+def combine(rows: torch.Tensor, slot_pos: torch.Tensor, weights=None) -> torch.Tensor:
+    """out[t] = sum_j weights[t, j] * rows[slot_pos[t, j]]: rows [P, H] bf16 in
+    send order -> [n, H] bf16 (fp32 sum; None weights = 1).  A negative position
+    adds nothing, nor does one beyond the rows, which also sets the device
+    error word."""
+    rows, slot_pos, weights = _combine_args(rows, slot_pos, weights)
+    (n, k), H, dev = slot_pos.shape, rows.shape[1], rows.device
+    out = torch.empty(n, H, dtype=torch.bfloat16, device=dev)
+    with _lib.on_device(dev):
+        _lib.check(_lib.load().mxg_ep_combine_rows(rows.data_ptr(), rows.shape[0], slot_pos.data_ptr(),
+                                                   _lib.ptr(weights), n, k, H, out.data_ptr(),
+                                                   _lib.stream_ptr(dev)), "mxg_ep_combine_rows")
+    return out
+
+
+def combine_bwd(dout: torch.Tensor, rows: torch.Tensor, slot_pos: torch.Tensor, weights=None, *,
+                need_rows: bool = True, need_weights: bool = True):
+    """Gradient of the combine out[t] = sum_j weights[t, j] * rows[slot_pos[t, j]]
+    (``ExpertParallel.combine_finish``; None weights = 1) from dout [n, H] bf16:
+    (drows like rows, dweights [n, topk] fp32; None where not needed).
+
+        drows[slot_pos[t, j]] = weights[t, j] * dout[t]
+        dweights[t, j]        = <dout[t], rows[slot_pos[t, j]]>
+
+    A negative position has no row (its dweights are 0); one beyond the rows
+    is skipped too and sets the device error word.  slot_pos names a row at
+    most once; a row that it does not name has gradient 0."""
+    rows, slot_pos, weights = _combine_args(rows, slot_pos, weights)
+    (n, k), (P, H), dev = slot_pos.shape, rows.shape, rows.device
+    if dout.dtype != torch.bfloat16 or dout.shape != (n, H) or dout.device != dev:
+        raise ValueError(f"dout must be a bf16 ({n}, {H}) tensor on {dev}")
+    dout = dout.contiguous()
+    drows = torch.empty_like(rows) if need_rows else None
+    dweights = torch.empty(n, k, dtype=torch.float32, device=dev) if need_weights else None
+    seen = torch.empty(P, dtype=torch.uint8, device=dev) if need_rows else None
+    with _lib.on_device(dev):
+        _lib.check(_lib.load().mxg_ep_combine_bwd(
+            dout.data_ptr(), rows.data_ptr(), slot_pos.data_ptr(), _lib.ptr(weights), n, k, H, P, _lib.ptr(drows),
+            _lib.ptr(dweights), _lib.ptr(seen), _lib.stream_ptr(dev)), "mxg_ep_combine_bwd")
+    return drows, dweights
 
 
 class gemm_sm_limit:

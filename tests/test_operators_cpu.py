@@ -1,0 +1,148 @@
+"""Argument checks of the router, the combine's gradient and AdamW, and the
+8-bit codes, on a machine without a GPU."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import adamw_oracle as ao
+
+
+def test_router_refuses_bad_arguments(mxg):
+    R = mxg.ops.router_topk
+    z = torch.zeros(4, 64)
+    with pytest.raises(ValueError, match="CUDA"):
+        R(z, 4)
+    with pytest.raises(ValueError, match="score"):
+        R(z, 4, score="relu")
+    with pytest.raises(ValueError, match="scale"):
+        R(z, 4, scale=0.0)
+    with pytest.raises(ValueError, match="group_score"):
+        R(z, 4, group_score="sum")
+    with pytest.raises(TypeError):
+        R(z.double(), 4)
+    with pytest.raises(TypeError):
+        R(z[0], 4)
+    with pytest.raises(ValueError, match="experts"):
+        R(torch.zeros(2, 385), 4)
+    with pytest.raises(ValueError, match="CUDA"):
+        mxg.ops.router_topk_bwd(z, z[:, :2], z[:, :2].int(), z[:, :2])
+    with pytest.raises(ValueError, match="scale"):
+        mxg.ops.router_topk_bwd(z, z[:, :2], z[:, :2].int(), z[:, :2], scale=float("inf"))
+
+
+def test_router_abi_refuses_bad_shapes(mxg):
+    L = mxg._lib.load()
+
+    def call(ld=64, dtype=1, n=4, E=64, k=4, score=0, groups=1, kept=1, gs=0, scale=1.0, z=16):
+        return L.mxg_router_topk(z, ld, dtype, n, E, k, score, None, groups, kept, gs, 1, scale, 16, 16, None)
+    assert call(n=0) == 0
+    assert call(n=-1) == 1 and call(E=0) == 1 and call(k=0) == 1 and call(dtype=3) == 1 and call(score=2) == 1
+    assert call(E=385, ld=385) == 2 and call(k=65) == 2 and call(k=33) == 2 and call(ld=63) == 2
+    assert call(groups=0) == 1 and call(groups=4, kept=5) == 1 and call(gs=2) == 1 and call(scale=-1.0) == 1
+    assert call(scale=float("nan")) == 1 and call(z=None) == 1
+    assert call(groups=5) == 2 and call(groups=64, kept=64) == 2
+    assert call(groups=16, kept=1, k=5) == 2                   # four experts are left
+    def bwd(ld=64, n=4, E=64, k=4, ld_out=64, scale=1.0, w=16):
+        return L.mxg_router_topk_bwd(16, ld, 1, n, E, k, 0, 1, scale, w, 16, 16, 16, ld_out, None)
+    assert bwd(n=0) == 0 and bwd(ld_out=60) == 2 and bwd(scale=0.0) == 1 and bwd(w=None) == 1 and bwd(k=65) == 2
+
+
+def test_combine_gradient_refuses_bad_arguments(mxg):
+    rows = torch.zeros(4, 16, dtype=torch.bfloat16)
+    pos = torch.zeros(2, 2, dtype=torch.int32)
+    for fn in (lambda: mxg.ops.combine_bwd(rows[:2], rows, pos), lambda: mxg.ops.combine(rows, pos)):
+        with pytest.raises(ValueError, match="CUDA"):
+            fn()
+    with pytest.raises(TypeError):
+        mxg.ops.combine_bwd(rows[:2], rows[:, :12], pos)
+    with pytest.raises(TypeError):
+        mxg.ops.combine_bwd(rows[:2], rows, pos.long())
+    L = mxg._lib.load()
+    call = lambda n=2, k=2, H=16, P=4, dout=16, rows=16, pos=16: L.mxg_ep_combine_bwd(
+        dout, rows, pos, None, n, k, H, P, 16, 16, None, None)
+    assert call(n=-1) == 1 and call(k=0) == 1 and call(H=12) == 2 and call(k=400) == 2 and call(P=-1) == 1
+    assert call(dout=None) == 1 and call(pos=None) == 1 and call(rows=24) == 3
+    assert L.mxg_ep_combine_bwd(16, 16, 16, None, 2, 2, 16, 4, None, None, None, None) == 0
+
+
+def test_adamw_refuses_bad_arguments(mxg):
+    A = mxg.optim.AdamW
+    p = torch.zeros(8)
+    with pytest.raises(ValueError, match="CUDA"):
+        A([p])
+    with pytest.raises(ValueError, match="at least one"):
+        A([])
+    with pytest.raises(ValueError, match="state_bits"):
+        A([p], state_bits=16)
+    with pytest.raises(ValueError, match="betas"):
+        A([p], betas=(0.9, 1.0))
+    with pytest.raises(ValueError, match="eps"):
+        A([p], eps=-1.0)
+    with pytest.raises(ValueError, match="decay"):
+        A([p], weight_decay=[0.1, 0.1])
+    with pytest.raises(ValueError, match="decay"):
+        A([p], weight_decay=-0.1)
+    with pytest.raises(TypeError):
+        A([p.half()])
+    with pytest.raises(ValueError, match="contiguous"):
+        A([torch.zeros(4, 4).t()])
+
+
+def test_adamw_abi_refuses_bad_arguments(mxg):
+    L = mxg._lib.load()
+    begin, grads, kinds = np.zeros(2, np.int64), np.array([16], np.uint64), np.array([1], np.int32)
+
+    def call(n=1, bits=32, m=16, ms=None, lr=1e-3, b1=0.9, b2=0.99, eps=1e-8, grads=grads, kinds=kinds, begin=begin,
+             step=16):
+        return L.mxg_adamw_step(16, n, 16, begin.ctypes.data, grads.ctypes.data, kinds.ctypes.data, bits, m, 16, ms,
+                                ms, None, step, 16, lr, None, b1, b2, eps, 0, None)
+    assert call(n=0) == 1 and call(bits=16) == 1 and call(m=None) == 1 and call(step=None) == 1
+    assert call(bits=8) == 1                                     # no scales
+    assert call(lr=-1.0) == 1 and call(b1=1.0) == 1 and call(b2=-0.1) == 1 and call(eps=float("nan")) == 1
+    assert call(kinds=np.array([2], np.int32)) == 1
+    assert call(grads=np.array([18], np.uint64)) == 3 and call(m=24) == 3
+    assert call(begin=np.array([3, 1], np.int64)) == 1
+    assert L.mxg_adamw_moments(16, 16, 16, 16, 100, 16, 16, None) == 2
+    assert L.mxg_adamw_moments(16, 16, 16, 16, 0, 16, 16, None) == 0
+    assert L.mxg_adamw_moments(16, None, 16, 16, 256, 16, 16, None) == 1
+
+
+def test_tensor_table_matches_the_header(mxg):
+    """The field offsets of mxg_adamw_tensor as a C compiler lays them out."""
+    e = mxg.optim._ENTRY
+    assert e.itemsize == 48
+    assert [e.fields[n][1] for n in ("param", "numel", "offset", "master", "decay", "kind", "first_chunk")] == \
+        [0, 8, 16, 24, 32, 36, 40]
+    text = open(mxg._lib.HEADER_PATH).read()
+    for name, value in (("MXG_ADAMW_BLOCK", 256), ("MXG_ADAMW_CHUNK", 4096), ("MXG_ROUTER_MAX_TOPK", 32),
+                        ("MXG_ROUTER_MAX_GROUPS", 32), ("MXG_EP_MAX_EXPERTS", 384)):
+        assert f"#define {name} {value}" in text
+        assert getattr(mxg._lib, name[4:]) == value
+
+
+@pytest.mark.parametrize("first", [True, False])
+def test_codes_round_without_bias(first):
+    """Mean of the decoded codes over many steps: within 5 standard errors."""
+    g = np.random.default_rng(0)
+    x = (g.standard_normal(256) * np.exp(g.uniform(-8, 0, 256))).astype(np.float32)
+    x = x if first else x * x
+    total, count = np.zeros(256), 3000
+    for t in range(count):
+        h, _ = ao.words(3, t, 512, 256)
+        codes, scale = ao.encode(x, ao.noise(h, first), first)
+        total += ao.decode(codes, scale, first)
+    gap = np.maximum(np.abs(x), scale[0] * 2.0 ** (-14 if first else -30)) / 8   # at most a code's step
+    # a second moment under the lowest code, 2^-33, is held at that code: up to one code above its mean
+    held = 0.0 if first else np.where(x < scale[0] * 2.0 ** -33, gap, 0.0)
+    assert np.all(np.abs(total / count - x) <= 5 * gap / 2 / np.sqrt(count) + 2.0 ** -16 * gap + held)
+
+
+def test_every_code_is_kept_by_a_round_trip():
+    codes = np.arange(256, dtype=np.uint8)
+    scale = np.ones(1, np.float32)
+    for first, top in ((True, 0x78), (False, 0xF8)):
+        kept = codes[(codes & (127 if first else 255)) <= top]
+        x = np.zeros(256, np.float32)
+        x[:kept.size] = ao.decode(np.resize(kept, 256), scale, first)[:kept.size]
+        again, s = ao.encode(x, np.zeros(256, np.uint64), first)
+        assert s[0] == 1.0 and np.array_equal(ao.decode(again, s, first)[:kept.size], x[:kept.size])
