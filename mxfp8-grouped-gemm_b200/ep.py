@@ -32,6 +32,7 @@ import torch
 import torch.distributed as dist
 
 from . import _lib
+from . import ops as device_ops
 
 
 class CudaEpOps:
@@ -85,6 +86,9 @@ class CudaEpOps:
                                          _lib.ptr(w), n, k, hidden, out.data_ptr(),
                                          _lib.stream_ptr(rows.device)), "mxg_ep_combine")
         return out
+
+    def combine_bwd(self, dout: torch.Tensor, rows: torch.Tensor, slot_pos: torch.Tensor, weights, n: int, k: int):
+        return device_ops.combine_bwd(dout, rows, slot_pos.view(n, k), weights, need_weights=weights is not None)
 
 
 class CudaP2POps:
@@ -392,6 +396,7 @@ class ExpertParallel:
         self.buffers = {}        # name -> PeerBuffer
         self.capacity = {}       # name -> rows
         self._flag = None
+        self._ret_need = None    # rows and row size of the return buffers
         self.marker = None       # optional callable(name): a timing mark on the current stream
         self.ce_streams = (self.world - 1 if ce_streams < 0 else ce_streams)
         self._ce = []            # the copy-engine streams, created on first use
@@ -556,7 +561,10 @@ class ExpertParallel:
         # return buffers ("ret", and any other combine_send names): every
         # rank's n*k rows in send order; sized like the receive buffers, from
         # the gathered counts, so every rank (re)allocates them together
-        self._ret_need = (int(sent.max()), max(n_cap * k, int(sent.max())), row_bytes)
+        # (never less than an earlier dispatch's, whose rows may still return)
+        need0, alloc0, rb0 = self._ret_need or (0, 0, row_bytes)
+        need0, alloc0 = (need0, alloc0) if rb0 == row_bytes else (0, 0)
+        self._ret_need = (max(int(sent.max()), need0), max(n_cap * k, int(sent.max()), alloc0), row_bytes)
         for name in [b for b in self.capacity if b not in ("x", "dy")] or ["ret"]:
             self._ensure_ret(name, x.device)
         slot_start, dest_base, group_rows, _, back_rank, back_row, ret_order = self.p2p.plan(
@@ -716,3 +724,32 @@ class ExpertParallel:
     def combine_finish(self, ret: torch.Tensor, plan: DispatchPlan, weights=None) -> torch.Tensor:
         """Second half of ``combine``: the weighted sum over each token's choices."""
         return self.ops.combine(ret, plan.slot_pos, weights, plan.n_tokens, plan.topk)
+
+    def combine_grad(self, dout: torch.Tensor, ret: torch.Tensor, plan: DispatchPlan, weights=None):
+        """Gradient of ``combine_finish``: from dout [n, H] and the rows ``ret``
+        that it summed (send order), the rows' gradient [n*k, H] in send order,
+        for ``dispatch_sent``, and that of the weights [n, k] (None without)."""
+        return self.ops.combine_bwd(dout, ret, plan.slot_pos, weights, plan.n_tokens, plan.topk)
+
+    def dispatch_sent(self, rows: torch.Tensor, plan: DispatchPlan, buffer: str = "dy",
+                      copy_engines: bool = False) -> torch.Tensor:
+        """``dispatch_like`` of rows [n*k, H'] that are in send order already, one
+        for each (token, choice): the gradient that ``combine_grad`` gives."""
+        if plan.back_rank is None:
+            recv_buf = self._a2a(rows, plan.recv_rows, plan.recv_splits, plan.send_splits)
+            return self.ops.gather(recv_buf, plan.idx, plan.idx.numel())
+        buf = self.buffers[buffer]
+        capacity, row_bytes = self.capacity[buffer]
+        if rows.shape[0] and rows.element_size() * rows[0].numel() != row_bytes:
+            self._barrier(rows.device)      # as in dispatch_like: nobody waits for this rank
+            raise ValueError("row size differs from the receive buffer's")
+        local = buf.view(plan.back_rank.numel(), rows)
+        self.p2p.zero_pad_rows(local, plan.back_rank)
+        if copy_engines:
+            self._copy_runs(rows, plan.runs_dispatch, buf.ptrs_host, capacity)
+        else:
+            order = torch.arange(plan.n_tokens * plan.topk, dtype=torch.int32, device=rows.device)
+            self.p2p.dispatch(rows, order, plan.slot_start, plan.dest_base, self.e_local, self.rank, buf.ptrs,
+                              capacity, self.p2p_max_blocks)
+        self._barrier(rows.device)
+        return local

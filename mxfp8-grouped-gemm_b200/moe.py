@@ -17,7 +17,18 @@ backward  dispatch dy along the same plan -> quantize (both directions) ->
           d_gate @ w1 + d_up @ w3) -> its rows back home, summed over each
           token's choices -> gate/up wgrad
 
-Weights are quantised once (static between optimiser steps).  With a comm
+``step`` takes the expert ids and router weights as given, and dy for every
+routed row.  ``forward`` and ``backward`` train the router too: ``forward``
+chooses the experts from logits (``Router``) and combines; ``backward`` takes the
+gradient of the combined output, from which the combine's gradient gives each
+routed row's (weighted) and the router weights', and these the logits':
+
+forward   route -> dispatch x -> ... as above ... -> combine
+backward  combine's gradient -> logits' gradient; rows in send order -> their
+          experts -> ... as above ... -> dx home
+
+Weights are quantised once and again by ``reencode`` after an optimiser step
+(``optim.AdamW``).  With a comm
 stream the dy dispatch runs under the forward GEMMs and the two returns under
 the backward GEMMs; only the x dispatch (and its count exchange) sits in front
 of the first GEMM.
@@ -25,6 +36,7 @@ of the first GEMM.
 from __future__ import annotations
 
 from contextlib import nullcontext
+from dataclasses import dataclass
 from typing import NamedTuple
 
 import torch
@@ -42,6 +54,51 @@ class LayerStep(NamedTuple):
     dw_gate_up: torch.Tensor
     dw_down: torch.Tensor
     plan: object
+
+
+@dataclass
+class Router:
+    """How a layer's tokens choose their experts: the arguments of
+    ``ops.router_topk`` (bias: fp32 [E] on the device, or None)."""
+    topk: int
+    score: str = "softmax"
+    bias: torch.Tensor | None = None
+    groups: int = 1
+    topk_groups: int | None = None
+    group_score: str = "max"
+    renormalize: bool = True
+    scale: float = 1.0
+
+    def __call__(self, logits: torch.Tensor):
+        """(weights [n, topk] fp32, ids [n, topk] int32) of logits [n, E]."""
+        return ops.router_topk(logits, self.topk, score=self.score, bias=self.bias, groups=self.groups,
+                               topk_groups=self.topk_groups, group_score=self.group_score,
+                               renormalize=self.renormalize, scale=self.scale)
+
+    def backward(self, logits, weights, ids, dweights) -> torch.Tensor:
+        """Gradient of the logits from that of the weights."""
+        return ops.router_topk_bwd(logits, weights, ids, dweights, score=self.score, renormalize=self.renormalize,
+                                   scale=self.scale)
+
+
+class RoutedForward(NamedTuple):
+    """Result of ``ExpertFFN.forward``: the combined output [n, H], the router's
+    weights and ids [n, topk], the dispatch plan, and what ``backward`` needs."""
+    out: torch.Tensor
+    weights: torch.Tensor
+    ids: torch.Tensor
+    plan: object
+    saved: tuple
+
+
+class RoutedGrads(NamedTuple):
+    """Result of ``ExpertFFN.backward``: the gradients of the token inputs [n, H]
+    (the experts' part; None when not computed), of the router's logits [n, E]
+    and of the local experts' weights."""
+    dx: torch.Tensor | None
+    dlogits: torch.Tensor
+    dw_gate_up: torch.Tensor
+    dw_down: torch.Tensor
 
 
 class ExpertFFN:
@@ -87,20 +144,7 @@ class ExpertFFN:
         if E != ep.e_local or E2 != E or H2 != H or I2 != 2 * I:
             raise ValueError("weights must be [E_local, 2I, H] and [E_local, H, I]")
         self.E, self.H, self.I = E, H, I
-        q, s = ops.quantize_rowwise(w_gate_up.reshape(E * 2 * I, H))
-        self.wgu = (q.view(E, 2 * I, H), s.view(E, 2 * I, H // 32))
-        q, s = ops.quantize_rowwise(w_down.reshape(E * H, I))
-        self.wd = (q.view(E, H, I), s.view(E, H, I // 32))
-        wdt = w_down.transpose(1, 2).contiguous()            # [E, I, H] for dh = dy . W_d
-        q, s = ops.quantize_rowwise(wdt.view(E * I, H))
-        self.wdt = (q.view(E, I, H), s.view(E, I, H // 32))
-        del wdt
-        self.wgut = None
-        if compute_dx:                                       # [E, H, 2I] for dx = dgu . W_gu
-            wgut = w_gate_up.transpose(1, 2).contiguous()
-            q, s = ops.quantize_rowwise(wgut.view(E * H, 2 * I))
-            self.wgut = (q.view(E, H, 2 * I), s.view(E, H, 2 * I // 32))
-            del wgut
+        self._encode(w_gate_up, w_down)
         self.comm = comm_stream
         self.ce = bool(copy_engines and comm_stream is not None)
         self.fused_return = bool(fused_return and ep.transport == "p2p")
@@ -115,6 +159,30 @@ class ExpertFFN:
             self.gemm_sms = 0
         self.marks = None           # optional list of (name, cuda event) for profiling
         self.trace = None           # optional dict: a step keeps its intermediates here
+
+    def _encode(self, w_gate_up, w_down):
+        E, H, I = self.E, self.H, self.I
+        q, s = ops.quantize_rowwise(w_gate_up.reshape(E * 2 * I, H))
+        self.wgu = (q.view(E, 2 * I, H), s.view(E, 2 * I, H // 32))
+        q, s = ops.quantize_rowwise(w_down.reshape(E * H, I))
+        self.wd = (q.view(E, H, I), s.view(E, H, I // 32))
+        wdt = w_down.transpose(1, 2).contiguous()            # [E, I, H] for dh = dy . W_d
+        q, s = ops.quantize_rowwise(wdt.view(E * I, H))
+        self.wdt = (q.view(E, I, H), s.view(E, I, H // 32))
+        del wdt
+        self.wgut = None
+        if self.compute_dx:                                  # [E, H, 2I] for dx = dgu . W_gu
+            wgut = w_gate_up.transpose(1, 2).contiguous()
+            q, s = ops.quantize_rowwise(wgut.view(E * H, 2 * I))
+            self.wgut = (q.view(E, H, 2 * I), s.view(E, H, 2 * I // 32))
+            del wgut
+
+    def reencode(self, w_gate_up: torch.Tensor, w_down: torch.Tensor) -> None:
+        """Quantise the weights again, after an optimiser step changed them."""
+        E, H, I = self.E, self.H, self.I
+        if tuple(w_gate_up.shape) != (E, 2 * I, H) or tuple(w_down.shape) != (E, H, I):
+            raise ValueError(f"weights must be [{E}, {2 * I}, {H}] and [{E}, {H}, {I}]")
+        self._encode(w_gate_up.detach(), w_down.detach())
 
     def _mark(self, name):
         if self.marks is not None:
@@ -291,6 +359,55 @@ class ExpertFFN:
                        gos_g=gos_g, dx_local=dx_local, ret=ret.clone(),
                        ret_dx=None if ret_dx is None else ret_dx.clone())
         return LayerStep(out, dx, dw_gu, dw_d, plan)
+
+    def forward(self, x, logits, router: Router) -> RoutedForward:
+        """Forward of one layer from router logits [n, E] (E over all ranks): x
+        [n, H] bf16 through its experts and the weighted combine.  Call
+        ``backward`` with the result, each rank in the same order.  (The options
+        split_experts and fused_return are ``step``'s.)"""
+        ep = self.ep
+        if logits.shape != (x.shape[0], ep.num_experts):
+            raise ValueError(f"logits must be [{x.shape[0]}, {ep.num_experts}], got {tuple(logits.shape)}")
+        weights, ids = router(logits)
+        x_local, plan = ep.dispatch(x, ids)
+        offs = plan.group_rows
+        xq, xs, ia_g, ias_g = ops.quantize_dual(x_local)
+        gu = self._fwd((xq, xs), self.wgu, offs)
+        hq, hs, ia_d, ias_d = ops.swiglu_quantize(gu)
+        y_local = self._fwd((hq, hs), self.wd, offs)
+        ret = ep.combine_send(y_local, plan, copy_engines=self.ce)
+        if plan.back_rank is not None:
+            ret = ret.clone()          # a view of the return buffer, which the next combine overwrites
+        out = ep.combine_finish(ret, plan, weights)
+        return RoutedForward(out, weights, ids, plan, (router, logits, gu, (ia_g, ias_g), (ia_d, ias_d), ret))
+
+    def backward(self, fwd: RoutedForward, dout: torch.Tensor) -> RoutedGrads:
+        """Gradients from dout [n, H] bf16, that of ``fwd.out``.  With a comm
+        stream the return of dx runs beside the gate/up weight gradient."""
+        ep, plan = self.ep, fwd.plan
+        router, logits, gu, ia_gate_up, ia_down, ret = fwd.saved
+        offs = plan.group_rows
+        main, comm = torch.cuda.current_stream(), self.comm
+        dsent, dweights = ep.combine_grad(dout, ret, plan, fwd.weights)
+        dlogits = router.backward(logits, fwd.weights, fwd.ids, dweights)
+        dy_local = ep.dispatch_sent(dsent, plan, copy_engines=self.ce)
+        dyq, dys, go_d, gos_d = ops.quantize_dual(dy_local)
+        dh = self._fwd((dyq, dys), self.wdt, offs)
+        dw_d = self._wgrad((go_d, gos_d), ia_down, offs)
+        dgq, dgs, go_g, gos_g = ops.swiglu_bwd_quantize(gu, dh, rowwise=self.compute_dx)
+        ret_dx = None
+        if self.compute_dx:
+            dx_local = self._fwd((dgq, dgs), self.wgut, offs)
+            if comm is not None:
+                comm.wait_stream(main)
+            with torch.cuda.stream(comm) if comm is not None else nullcontext():
+                ret_dx = ep.combine_send(dx_local, plan, buffer="ret_dx", copy_engines=self.ce)
+        with ops.gemm_sm_limit(self.gemm_sms if self.compute_dx else 0):
+            dw_gu = self._wgrad((go_g, gos_g), ia_gate_up, offs)
+        if comm is not None:
+            main.wait_stream(comm)     # later uses of either stream's memory come after this
+        dx = ep.combine_finish(ret_dx, plan, None) if ret_dx is not None else None
+        return RoutedGrads(dx, dlogits, dw_gu, dw_d)
 
     def gemm_flops(self, plan) -> dict:
         """Algorithmic FLOPs of the step's grouped GEMMs on real rows."""
