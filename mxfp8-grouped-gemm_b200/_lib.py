@@ -5,7 +5,6 @@ functions below raise; there is no CPU or library fallback.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 import re
@@ -171,13 +170,19 @@ def stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-_SAME_DEVICE = contextlib.nullcontext()
-
-
-def on_device(device: torch.device):
-    """Context in which ``device`` is the current one: the C ABI launches on
-    the current device, and a tensor may lie on another."""
-    return _SAME_DEVICE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def launch(name: str, device: torch.device, *args) -> None:
+    """Call entry point ``name`` with ``args`` and the current stream of
+    ``device``, made the current device for the call (the C ABI launches on
+    the current one)."""
+    fn = getattr(_lib or load(), name)
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if code != MXG_OK:
+        raise MxgError(code, name)
 
 
 def ptr(t) -> int | None:

@@ -355,11 +355,9 @@ def router_topk(logits: torch.Tensor, topk: int, *, score: str = "softmax", bias
             raise ValueError("bias and logits must be on one device")
     weights = torch.empty(n, topk, dtype=torch.float32, device=dev)
     ids = torch.empty(n, topk, dtype=torch.int32, device=dev)
-    with _lib.on_device(dev):
-        _lib.check(_lib.load().mxg_router_topk(
-            logits.data_ptr(), ld, _LOGITS[logits.dtype], n, E, topk, code, _lib.ptr(bias), groups, topk_groups,
-            _GROUP_SCORES[group_score], renormalize, scale, weights.data_ptr(), ids.data_ptr(),
-            _lib.stream_ptr(dev)), "mxg_router_topk")
+    _lib.launch("mxg_router_topk", dev, logits.data_ptr(), ld, _LOGITS[logits.dtype], n, E, topk, code,
+                _lib.ptr(bias), groups, topk_groups, _GROUP_SCORES[group_score], renormalize, scale,
+                weights.data_ptr(), ids.data_ptr())
     return weights, ids
 
 
@@ -384,11 +382,8 @@ def router_topk_bwd(logits: torch.Tensor, weights: torch.Tensor, ids: torch.Tens
     if not weights.device == ids.device == dweights.device == dev:
         raise ValueError("logits, weights, ids and dweights must be on one device")
     out = torch.empty(n, E, dtype=logits.dtype, device=dev)
-    with _lib.on_device(dev):
-        _lib.check(_lib.load().mxg_router_topk_bwd(
-            logits.data_ptr(), ld, _LOGITS[logits.dtype], n, E, shape[1], code, renormalize, scale,
-            weights.data_ptr(), ids.data_ptr(), dweights.data_ptr(), out.data_ptr(), E, _lib.stream_ptr(dev)),
-            "mxg_router_topk_bwd")
+    _lib.launch("mxg_router_topk_bwd", dev, logits.data_ptr(), ld, _LOGITS[logits.dtype], n, E, shape[1], code,
+                renormalize, scale, weights.data_ptr(), ids.data_ptr(), dweights.data_ptr(), out.data_ptr(), E)
     return out
 
 
@@ -415,10 +410,8 @@ def combine(rows: torch.Tensor, slot_pos: torch.Tensor, weights=None) -> torch.T
     rows, slot_pos, weights = _combine_args(rows, slot_pos, weights)
     (n, k), H, dev = slot_pos.shape, rows.shape[1], rows.device
     out = torch.empty(n, H, dtype=torch.bfloat16, device=dev)
-    with _lib.on_device(dev):
-        _lib.check(_lib.load().mxg_ep_combine_rows(rows.data_ptr(), rows.shape[0], slot_pos.data_ptr(),
-                                                   _lib.ptr(weights), n, k, H, out.data_ptr(),
-                                                   _lib.stream_ptr(dev)), "mxg_ep_combine_rows")
+    _lib.launch("mxg_ep_combine_rows", dev, rows.data_ptr(), rows.shape[0], slot_pos.data_ptr(), _lib.ptr(weights),
+                n, k, H, out.data_ptr())
     return out
 
 
@@ -442,10 +435,8 @@ def combine_bwd(dout: torch.Tensor, rows: torch.Tensor, slot_pos: torch.Tensor, 
     drows = torch.empty_like(rows) if need_rows else None
     dweights = torch.empty(n, k, dtype=torch.float32, device=dev) if need_weights else None
     seen = torch.empty(P, dtype=torch.uint8, device=dev) if need_rows else None
-    with _lib.on_device(dev):
-        _lib.check(_lib.load().mxg_ep_combine_bwd(
-            dout.data_ptr(), rows.data_ptr(), slot_pos.data_ptr(), _lib.ptr(weights), n, k, H, P, _lib.ptr(drows),
-            _lib.ptr(dweights), _lib.ptr(seen), _lib.stream_ptr(dev)), "mxg_ep_combine_bwd")
+    _lib.launch("mxg_ep_combine_bwd", dev, dout.data_ptr(), rows.data_ptr(), slot_pos.data_ptr(), _lib.ptr(weights),
+                n, k, H, P, _lib.ptr(drows), _lib.ptr(dweights), _lib.ptr(seen))
     return drows, dweights
 
 

@@ -154,13 +154,11 @@ class AdamW:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("a tensor moved since the last step: take one step before the capture")
             self._lay_out()
-        with _lib.on_device(self.device):
-            _lib.check(_lib.load().mxg_adamw_step(
-                self._table.data_ptr(), len(params), self._chunks.data_ptr(), self._chunk_begin.ctypes.data,
-                ptrs.ctypes.data, kinds.ctypes.data, self.state_bits, self.exp_avg.data_ptr(),
-                self.exp_avg_sq.data_ptr(), _lib.ptr(self.exp_avg_scale), _lib.ptr(self.exp_avg_sq_scale),
-                _lib.ptr(self.master), self._step.data_ptr(), self._done.data_ptr(), lr, lr_ptr, self.betas[0],
-                self.betas[1], self.eps, self.seed, _lib.stream_ptr(self.device)), "mxg_adamw_step")
+        _lib.launch("mxg_adamw_step", self.device, self._table.data_ptr(), len(params), self._chunks.data_ptr(),
+                    self._chunk_begin.ctypes.data, ptrs.ctypes.data, kinds.ctypes.data, self.state_bits,
+                    self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), _lib.ptr(self.exp_avg_scale),
+                    _lib.ptr(self.exp_avg_sq_scale), _lib.ptr(self.master), self._step.data_ptr(),
+                    self._done.data_ptr(), lr, lr_ptr, self.betas[0], self.betas[1], self.eps, self.seed)
         tracked = [p for p in params if p.requires_grad]
         if tracked:                                # autograd sees the change in place
             torch.autograd.graph.increment_version(tracked)
@@ -172,11 +170,8 @@ class AdamW:
             return self.exp_avg, self.exp_avg_sq
         n, dev = self.exp_avg.numel(), self.device
         avg, sq = torch.empty(n, device=dev), torch.empty(n, device=dev)
-        with _lib.on_device(dev):
-            _lib.check(_lib.load().mxg_adamw_moments(
-                self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), self.exp_avg_scale.data_ptr(),
-                self.exp_avg_sq_scale.data_ptr(), n, avg.data_ptr(), sq.data_ptr(), _lib.stream_ptr(dev)),
-                "mxg_adamw_moments")
+        _lib.launch("mxg_adamw_moments", dev, self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(),
+                    self.exp_avg_scale.data_ptr(), self.exp_avg_sq_scale.data_ptr(), n, avg.data_ptr(), sq.data_ptr())
         return avg, sq
 
     def view(self, flat: torch.Tensor, i: int) -> torch.Tensor:

@@ -70,6 +70,39 @@ def test_groups(mxg, cuda_dev, E, groups, kept, k, group_score, dtype):
         _check(mxg, z, k, score=score, bias=bias, renormalize=False, **how)
 
 
+@pytest.mark.parametrize("E,groups,kept", [(137, 1, 1), (160, 5, 2), (192, 3, 2), (256, 1, 1), (256, 8, 4), (256, 2, 1),
+                                           (257, 1, 1), (384, 1, 1), (384, 12, 4)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_long_batches(mxg, cuda_dev, E, groups, kept, dtype):
+    """Enough tokens for the layout of several tokens a warp at every E."""
+    z = _logits(8203, E, dtype, E + groups, cuda_dev)
+    z[17] = -float("inf")
+    z[18, 3:] = -float("inf")
+    z[:, E // 2] = -float("inf")
+    bias = torch.randn(E, device=cuda_dev, generator=torch.Generator(cuda_dev).manual_seed(E)) * 0.05
+    how = dict(groups=groups, topk_groups=kept)
+    for score in ("softmax", "sigmoid"):
+        _check(mxg, z, 8, score=score, **how)
+        _check(mxg, z, 5, score=score, renormalize=False, group_score="top2", **how)
+        _check(mxg, z, 8, score=score, bias=bias, group_score="top2", renormalize=False, **how)
+        _check(mxg, z, 7, score=score, bias=bias * 40, **how)
+    _check(mxg, torch.zeros_like(z), 8, score="sigmoid", bias=bias * 0, **how)
+
+
+@pytest.mark.parametrize("n", [64, 4200])
+@pytest.mark.parametrize("many", [12, 200])
+def test_long_rows_of_near_ties(mxg, cuda_dev, n, many):
+    """s + bias of `many` of 256 experts meets at 1 to the last places of fp32."""
+    g = torch.Generator(device=cuda_dev).manual_seed(many)
+    bias = torch.rand(256, generator=g, device=cuda_dev) * 0.5 + 0.2
+    s = 1 - bias.double() + torch.randn(n, 256, generator=g, device=cuda_dev, dtype=torch.float64) * 4e-8
+    s[:, torch.randperm(256, generator=g, device=cuda_dev)[many:]] *= 0.5
+    z = torch.log(s / (1 - s)).float()
+    _check(mxg, z, 8, score="sigmoid", bias=bias)
+    _check(mxg, z, 3, score="sigmoid", bias=bias, groups=8, topk_groups=4, group_score="top2")
+    _check(mxg, z, 3, score="sigmoid", bias=bias, groups=8, topk_groups=4)
+
+
 def test_ties_go_to_the_lowest_index(mxg, cuda_dev):
     z = torch.zeros(5, 256, device=cuda_dev)
     z[1, 200:] = 1.0
