@@ -267,12 +267,10 @@ MXG_API int mxg_ep_combine_rows(const void* rows, int64_t n_rows, const int32_t*
  * 1).  A negative position has no row: its dweights are 0.  One that is >=
  * n_rows is skipped too and sets the device error word to
  * MXG_ERR_INVALID_ARGUMENT.  slot_pos names a position at most once, as
- * mxg_ep_route gives it.  Rows of drows that it does not name become zero with
- * seen (n_rows bytes of workspace), and are left as they were when it is null. */
+ * mxg_ep_route gives it; rows of drows that it does not name become zero. */
 MXG_API int mxg_ep_combine_bwd(const void* dout, const void* rows, const int32_t* slot_pos,
                                const float* weights, int64_t n_tokens, int topk, int64_t hidden,
-                               int64_t n_rows, void* drows, float* dweights, uint8_t* seen,
-                               void* stream);
+                               int64_t n_rows, void* drows, float* dweights, void* stream);
 
 /* h = silu(g) * u for gu rows [g (inter) | u (inter)], bf16 (the gate/up ->
  * down activation of the expert FFN, e2e_bench.py:56-61). */

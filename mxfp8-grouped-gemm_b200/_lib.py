@@ -73,7 +73,7 @@ _PROTOS = {
     "mxg_ep_regroup": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp]),
     "mxg_ep_combine": (_c_int, [_vp, _vp, _vp, _c_i64, _c_int, _c_i64, _vp, _vp]),
     "mxg_ep_combine_rows": (_c_int, [_vp, _c_i64, _vp, _vp, _c_i64, _c_int, _c_i64, _vp, _vp]),
-    "mxg_ep_combine_bwd": (_c_int, [_vp, _vp, _vp, _vp, _c_i64, _c_int, _c_i64, _c_i64, _vp, _vp, _vp, _vp]),
+    "mxg_ep_combine_bwd": (_c_int, [_vp, _vp, _vp, _vp, _c_i64, _c_int, _c_i64, _c_i64, _vp, _vp, _vp]),
     "mxg_router_topk": (_c_int, [_vp, _c_i64, _c_int, _c_i64, _c_int, _c_int, _c_int, _vp, _c_int, _c_int,
                                  _c_int, _c_int, _c_f32, _vp, _vp, _vp]),
     "mxg_router_topk_bwd": (_c_int, [_vp, _c_i64, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_f32, _vp,
@@ -167,7 +167,8 @@ def raise_device_error() -> None:
 
 
 def stream_ptr(device: torch.device | None = None) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    index = device.index if device is not None else None
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def launch(name: str, device: torch.device, *args) -> None:

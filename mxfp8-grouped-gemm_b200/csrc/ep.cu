@@ -226,39 +226,94 @@ __global__ void __launch_bounds__(128) combine_kernel(const __nv_bfloat16* __res
 
 // Gradient of combine.  One block a token: its dout row stays in registers
 // (U vectors of 8 a thread) while the token's k rows pass by once, each giving
-// a partial dot product and taking the row's gradient.  Bound by HBM (k rows
-// in, k rows out, one dout row).  The dot products are summed in a fixed
-// order: over a thread's columns, over the warp, over the warps.
+// a partial dot product and taking the row's gradient; the next row is on its
+// way meanwhile.  Bound by HBM (k rows in, k rows out, one dout row).  The dot
+// products are summed in a fixed order: over a thread's columns, over the
+// warp, over the warps.  The first `fill_blocks` blocks write zeros to the
+// rows that no position names: each marks the positions of its kFillRows rows
+// that it finds in the whole table (4 bytes a choice beside 4 * hidden).
+constexpr int kFillRows = 32768;
+
+__device__ __forceinline__ void zero_unnamed_rows(const int32_t* __restrict__ inv, int64_t n, int64_t first,
+                                                  int64_t n_rows, int64_t vecs, uint4* __restrict__ rows,
+                                                  uint32_t* named) {
+  const int count = int(min(int64_t(kFillRows), n_rows - first));
+  for (int i = threadIdx.x; i < kFillRows / 32; i += blockDim.x) named[i] = 0;
+  __syncthreads();
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
+    const int64_t p = inv[i] - first;
+    if (p >= 0 && p < count) atomicOr(&named[p >> 5], 1u << (p & 31));
+  }
+  __syncthreads();
+  for (int i = 0; i < (count + 31) / 32; ++i) {
+    uint32_t left = ~named[i];
+    if (i == count / 32) left &= (1u << (count & 31)) - 1u;
+    for (; left; left &= left - 1) {
+      uint4* row = rows + (first + i * 32 + __ffs(left) - 1) * vecs;
+      for (int64_t c = threadIdx.x; c < vecs; c += blockDim.x) row[c] = make_uint4(0, 0, 0, 0);
+    }
+  }
+}
+
 template <int U>
 __global__ void __launch_bounds__(256) combine_bwd_kernel(const __nv_bfloat16* __restrict__ dout,
                                                           const __nv_bfloat16* __restrict__ rows,
                                                           const int32_t* __restrict__ inv,
                                                           const float* __restrict__ w, int topk, int64_t hidden,
                                                           int64_t n_rows, __nv_bfloat16* __restrict__ drows,
-                                                          float* __restrict__ dw, uint8_t* __restrict__ seen,
-                                                          int* err) {
+                                                          float* __restrict__ dw, int64_t n_tokens,
+                                                          int fill_blocks, int* err) {
   extern __shared__ float part[];  // [topk][warps]
-  const int64_t t = blockIdx.x;
+  __shared__ uint32_t named[kFillRows / 32];
+  if (int(blockIdx.x) < fill_blocks) {
+    zero_unnamed_rows(inv, n_tokens * topk, int64_t(blockIdx.x) * kFillRows, n_rows, hidden / 8,
+                      reinterpret_cast<uint4*>(drows), named);
+    return;
+  }
+  const int64_t t = int64_t(blockIdx.x) - fill_blocks;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int64_t vecs = hidden / 8;
-  for (int64_t c0 = 0; c0 < vecs; c0 += int64_t(U) * blockDim.x) {
-    uint4 d[U];
+  inv += t * topk;
+  for (int64_t c0 = threadIdx.x; c0 - threadIdx.x < vecs; c0 += int64_t(U) * blockDim.x) {
+    auto load = [&](const __nv_bfloat16* row, uint4(&x)[U]) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t c = c0 + u * int64_t(blockDim.x) + threadIdx.x;
-      d[u] = c < vecs ? __ldg(reinterpret_cast<const uint4*>(dout + t * hidden) + c) : make_uint4(0, 0, 0, 0);
-    }
+      for (int u = 0; u < U; ++u) {
+        const int64_t c = c0 + u * int64_t(blockDim.x);
+        x[u] = c < vecs ? __ldcs(reinterpret_cast<const uint4*>(row) + c) : make_uint4(0, 0, 0, 0);
+      }
+    };
+    uint4 d[U], next[U];
+    int64_t p_next = inv[0];
+    if (dw && p_next >= 0 && p_next < n_rows) load(rows + p_next * hidden, next);
+    load(dout + t * hidden, d);
     for (int j = 0; j < topk; ++j) {
-      const int64_t p = inv[t * topk + j];
-      float dot = 0.0f;
-      if (p >= 0 && p < n_rows) {
-        if (dw) {
-          uint4 x[U];
+      const int64_t p = p_next;
+      const bool real = p >= 0 && p < n_rows;
+      uint4 x[U];
 #pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const int64_t c = c0 + u * int64_t(blockDim.x) + threadIdx.x;
-            x[u] = c < vecs ? __ldcs(reinterpret_cast<const uint4*>(rows + p * hidden) + c) : make_uint4(0, 0, 0, 0);
-          }
+      for (int u = 0; u < U; ++u) x[u] = next[u];
+      if (j + 1 < topk) {
+        p_next = inv[j + 1];
+        if (dw && p_next >= 0 && p_next < n_rows) load(rows + p_next * hidden, next);
+      }
+      if (drows && real) {
+        const float wj = w ? w[t * topk + j] : 1.0f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int64_t c = c0 + u * int64_t(blockDim.x);
+          const uint32_t* a = reinterpret_cast<const uint32_t*>(&d[u]);
+          uint4 o;
+          uint32_t* b = reinterpret_cast<uint32_t*>(&o);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) b[q] = pack2_bf16(wj * bf16_lo(a[q]), wj * bf16_hi(a[q]));
+          if (c < vecs) __stcs(reinterpret_cast<uint4*>(drows + p * hidden) + c, o);
+        }
+      }
+      if (p >= n_rows && c0 == 0) atomicCAS(err, 0, MXG_ERR_INVALID_ARGUMENT);
+      if (dw) {
+        float dot = 0.0f;
+        if (real) {
 #pragma unroll
           for (int u = 0; u < U; ++u) {
             const uint32_t* a = reinterpret_cast<const uint32_t*>(&d[u]);
@@ -270,27 +325,9 @@ __global__ void __launch_bounds__(256) combine_bwd_kernel(const __nv_bfloat16* _
             }
           }
         }
-        if (drows) {
-          if (seen && c0 == 0 && threadIdx.x == 0) seen[p] = 1;
-          const float wj = w ? w[t * topk + j] : 1.0f;
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const int64_t c = c0 + u * int64_t(blockDim.x) + threadIdx.x;
-            const uint32_t* a = reinterpret_cast<const uint32_t*>(&d[u]);
-            uint4 o;
-            uint32_t* b = reinterpret_cast<uint32_t*>(&o);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) b[q] = pack2_bf16(wj * bf16_lo(a[q]), wj * bf16_hi(a[q]));
-            if (c < vecs) __stcs(reinterpret_cast<uint4*>(drows + p * hidden) + c, o);
-          }
-        }
-      } else if (p >= n_rows && threadIdx.x == 0) {
-        atomicCAS(err, 0, MXG_ERR_INVALID_ARGUMENT);
-      }
-      if (dw) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-        if (lane == 0) part[j * warps + warp] = c0 == 0 ? dot : part[j * warps + warp] + dot;
+        if (lane == 0) part[j * warps + warp] = c0 == threadIdx.x ? dot : part[j * warps + warp] + dot;
       }
     }
   }
@@ -300,19 +337,6 @@ __global__ void __launch_bounds__(256) combine_bwd_kernel(const __nv_bfloat16* _
     float s = 0.0f;
     for (int q = 0; q < warps; ++q) s += part[j * warps + q];
     dw[t * topk + j] = s;
-  }
-}
-
-// Zeros in the rows that combine_bwd_kernel did not write.
-__global__ void __launch_bounds__(256) zero_unseen_rows_kernel(const uint8_t* __restrict__ seen, int64_t n_rows,
-                                                               int64_t vecs, uint4* __restrict__ rows) {
-  for (int64_t r0 = int64_t(blockIdx.x) * 256; r0 < n_rows; r0 += int64_t(gridDim.x) * 256) {
-    const bool zero = r0 + threadIdx.x < n_rows && !seen[r0 + threadIdx.x];
-    if (!__syncthreads_or(zero)) continue;
-    for (int64_t r = r0; r < min(n_rows, r0 + 256); ++r) {
-      if (seen[r]) continue;
-      for (int64_t c = threadIdx.x; c < vecs; c += 256) rows[r * vecs + c] = make_uint4(0, 0, 0, 0);
-    }
   }
 }
 
@@ -473,7 +497,7 @@ extern "C" int mxg_ep_combine_rows(const void* rows, int64_t n_rows, const int32
 
 extern "C" int mxg_ep_combine_bwd(const void* dout, const void* rows, const int32_t* slot_pos, const float* weights,
                                   int64_t n_tokens, int topk, int64_t hidden, int64_t n_rows, void* drows,
-                                  float* dweights, uint8_t* seen, void* stream) {
+                                  float* dweights, void* stream) {
   if (n_tokens < 0 || topk < 1 || hidden < 0 || n_rows < 0) return MXG_ERR_INVALID_ARGUMENT;
   if (hidden % 8 != 0 || topk > MXG_EP_MAX_EXPERTS || n_tokens > INT32_MAX) return MXG_ERR_BAD_SHAPE;
   if (!drows && !dweights) return MXG_OK;
@@ -483,7 +507,7 @@ extern "C" int mxg_ep_combine_bwd(const void* dout, const void* rows, const int3
     if (dweights && n_tokens &&
         cudaMemsetAsync(dweights, 0, sizeof(float) * n_tokens * topk, (cudaStream_t)stream) != cudaSuccess)
       return MXG_ERR_CUDA;
-    if (drows && seen && n_rows && hidden &&
+    if (drows && n_rows && hidden &&
         cudaMemsetAsync(drows, 0, 2 * n_rows * hidden, (cudaStream_t)stream) != cudaSuccess)
       return MXG_ERR_CUDA;
     return MXG_OK;
@@ -494,19 +518,21 @@ extern "C" int mxg_ep_combine_bwd(const void* dout, const void* rows, const int3
   int* err = device_error_word();
   if (!err) return MXG_ERR_CUDA;
   const int64_t vecs = hidden / 8;
-  const int threads = int(std::min<int64_t>(256, (vecs + 31) / 32 * 32));
+  // Threads a block, each with 2 vectors of a row: few, so that many tokens
+  // are in flight, where there are tokens enough.  us at 64 / 128 / 256:
+  // 16384 x 8 x 7168 626 / 651 / 681 (98% of the copy rate at 64), 5001 x 2 x
+  // 14336 127 / 118 / 121; with 1 vector 790, with 4 620 / 663 / 724.
+  const int most = n_tokens >= 8192 ? 64 : n_tokens >= 1024 ? 128 : 256;
+  const int u = vecs <= most ? 1 : 2;
+  const int64_t passes = (vecs + u * most - 1) / (u * most);
+  const int threads = int((vecs + u * passes * 32 - 1) / (u * passes * 32)) * 32;
   const size_t smem = sizeof(float) * size_t(topk) * (threads / 32);
-  if (seen && drows && n_rows && cudaMemsetAsync(seen, 0, n_rows, (cudaStream_t)stream) != cudaSuccess)
-    return MXG_ERR_CUDA;
-  auto* kernel = vecs <= 256 ? combine_bwd_kernel<1> : vecs <= 512 ? combine_bwd_kernel<2> : combine_bwd_kernel<4>;
-  kernel<<<unsigned(n_tokens), threads, smem, (cudaStream_t)stream>>>(
+  const int64_t fill = drows ? (n_rows + kFillRows - 1) / kFillRows : 0;
+  if (n_tokens + fill > INT32_MAX) return MXG_ERR_BAD_SHAPE;
+  auto* kernel = u == 1 ? combine_bwd_kernel<1> : combine_bwd_kernel<2>;
+  kernel<<<unsigned(n_tokens + fill), threads, smem, (cudaStream_t)stream>>>(
       reinterpret_cast<const __nv_bfloat16*>(dout), reinterpret_cast<const __nv_bfloat16*>(rows), slot_pos, weights,
-      topk, hidden, n_rows, reinterpret_cast<__nv_bfloat16*>(drows), dweights, seen, err);
-  if (seen && drows && n_rows) {
-    const int64_t blocks = std::min<int64_t>((n_rows + 255) / 256, int64_t(num_sms()) * 4);
-    zero_unseen_rows_kernel<<<unsigned(blocks), 256, 0, (cudaStream_t)stream>>>(seen, n_rows, vecs,
-                                                                              reinterpret_cast<uint4*>(drows));
-  }
+      topk, hidden, n_rows, reinterpret_cast<__nv_bfloat16*>(drows), dweights, n_tokens, int(fill), err);
   return cuda_status(cudaGetLastError());
 }
 

@@ -434,9 +434,8 @@ def combine_bwd(dout: torch.Tensor, rows: torch.Tensor, slot_pos: torch.Tensor, 
     dout = dout.contiguous()
     drows = torch.empty_like(rows) if need_rows else None
     dweights = torch.empty(n, k, dtype=torch.float32, device=dev) if need_weights else None
-    seen = torch.empty(P, dtype=torch.uint8, device=dev) if need_rows else None
     _lib.launch("mxg_ep_combine_bwd", dev, dout.data_ptr(), rows.data_ptr(), slot_pos.data_ptr(), _lib.ptr(weights),
-                n, k, H, P, _lib.ptr(drows), _lib.ptr(dweights), _lib.ptr(seen))
+                n, k, H, P, _lib.ptr(drows), _lib.ptr(dweights))
     return drows, dweights
 
 

@@ -59,10 +59,10 @@ def test_combine_gradient_refuses_bad_arguments(mxg):
         mxg.ops.combine_bwd(rows[:2], rows, pos.long())
     L = mxg._lib.load()
     call = lambda n=2, k=2, H=16, P=4, dout=16, rows=16, pos=16: L.mxg_ep_combine_bwd(
-        dout, rows, pos, None, n, k, H, P, 16, 16, None, None)
+        dout, rows, pos, None, n, k, H, P, 16, 16, None)
     assert call(n=-1) == 1 and call(k=0) == 1 and call(H=12) == 2 and call(k=400) == 2 and call(P=-1) == 1
     assert call(dout=None) == 1 and call(pos=None) == 1 and call(rows=24) == 3
-    assert L.mxg_ep_combine_bwd(16, 16, 16, None, 2, 2, 16, 4, None, None, None, None) == 0
+    assert L.mxg_ep_combine_bwd(16, 16, 16, None, 2, 2, 16, 4, None, None, None) == 0
 
 
 def test_adamw_refuses_bad_arguments(mxg):

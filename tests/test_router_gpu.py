@@ -323,6 +323,18 @@ def test_combine_gradient(mxg, cuda_dev, n, k, H, extra, missing):
         assert torch.equal(mxg.ops.combine_bwd(dout, rows, pos, weights, need_rows=False)[1], dw)
 
 
+def test_combine_gradient_of_rows_that_nothing_names(mxg, cuda_dev):
+    """More rows than one block looks after, most of them named by nothing."""
+    for n, k, P, missing in ((40, 2, 100_003, 5), (16_500, 2, 33_000, 7), (9000, 8, 72_001, 0)):
+        dout, rows, pos, w = _combine_inputs(n, k, 64, P, n, cuda_dev, missing)
+        drows, dw = mxg.ops.combine_bwd(dout, rows, pos, w)
+        want = torch.zeros_like(rows)
+        ok = pos >= 0
+        t = torch.arange(n, device=cuda_dev)[:, None].expand(n, k)[ok]
+        want[pos[ok].long()] = (w[ok][:, None] * dout[t].float()).to(torch.bfloat16)
+        assert torch.equal(drows, want) and torch.all(dw[~ok] == 0)
+
+
 def test_combine_gradient_skips_positions_beyond_the_rows(mxg, cuda_dev):
     dout, rows, pos, w = _combine_inputs(16, 2, 64, 32, 1, cuda_dev)
     lost = int(pos[3, 1])
