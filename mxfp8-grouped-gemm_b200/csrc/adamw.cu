@@ -1,8 +1,8 @@
 // One AdamW step over many tensors for sm_100a.
 //
-// The tensors are cut into chunks of MXG_ADAMW_CHUNK elements; a persistent
-// grid walks the chunk table, a warp taking 256 elements at a time (8 a lane,
-// the block that shares one scale of the 8-bit moments).  Bound by HBM: every
+// The tensors are cut into chunks of MXG_ADAMW_CHUNK elements; every block takes
+// an equal run of the chunk table, a warp 256 elements at a time (8 a lane, the
+// block that shares one scale of the 8-bit moments).  Bound by HBM: every
 // array passes by once, in 16-byte accesses.
 //
 // The moments are rounded operation by operation (no fused multiply-adds), so
@@ -63,51 +63,111 @@ __device__ __forceinline__ uint32_t element_bits(uint32_t kb, uint32_t j) {
 }
 __device__ __forceinline__ uint32_t more_bits(uint32_t h) { return mix(h ^ kAdd, kM1); }
 
-// 8-bit codes: the bits of a float whose exponent field is small enough for
-// the code to be its bits 20 and up; denormals continue the grid to 0.
-__device__ __forceinline__ float decode_m(uint32_t c, float scale) {
-  const float x = __uint_as_float((c & 127u) << 20) * 0x1p112f * scale;
-  return (c & 128u) ? -x : x;
+// 8-bit codes are bits 20 and up of a float whose exponent field is small
+// enough (denormals continue the grid to 0).  The first moment's are e4m3 codes
+// (times 2^-8), which the conversion instruction decodes two at a time; the
+// second's become floats as they are.  A scale of 2^30 and more, whose product
+// with 2^96 would overflow, takes two products (the same value).
+__device__ __forceinline__ void decode_m(uint32_t codes, float scale, float (&x)[8], int at) {
+  const float by = scale * 0x1p-8f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const __half2_raw r =
+        __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(h ? codes >> 16 : codes & 0xFFFFu), __NV_E4M3);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r));
+    x[at + 2 * h] = f.x * by;
+    x[at + 2 * h + 1] = f.y * by;
+  }
 }
-__device__ __forceinline__ float decode_v(uint32_t c, float scale) {
-  return __uint_as_float(c << 20) * 0x1p96f * scale;
+__device__ __forceinline__ void decode_v(uint32_t codes, float scale, float (&x)[8], int at) {
+  const bool big = scale >= 0x1p30f;
+  const float by = big ? 0x1p96f : scale * 0x1p96f, more = big ? scale : 1.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t u = i < 3 ? codes << (20 - 8 * i) : codes >> 4;
+    x[at + i] = __uint_as_float(u & 0x0FF00000u) * by;
+  }
+  if (big) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[at + i] *= more;
+  }
 }
+// The code as the top byte, sign apart; noise: 16 random bits, in bits 8 to 23.
+// (A NaN or infinity spills over, into a block whose scale is one too.)  The
+// two products are spelled out: nvcc 12.9 at -O3 drops what follows a plain
+// product by 2^-112 here and yields codes of 0.
 __device__ __forceinline__ uint32_t encode_m(float x, float inv, uint32_t noise) {
-  const float y = fabsf(x) * inv * 0x1p-112f;
-  const uint32_t c = min((__float_as_uint(y) + noise) >> 20, 127u);
-  return c | (x < 0.0f ? 128u : 0u);
+  const uint32_t t = __float_as_uint(__fmul_rn(__fmul_rn(fabsf(x), inv), 0x1p-112f)) * 16u + noise;
+  return (t & 0x7FFFFFFFu) | (__float_as_uint(x) & 0x80000000u);
 }
 __device__ __forceinline__ uint32_t encode_v(float x, float inv, uint32_t noise) {
-  const float y = x * inv * 0x1p-96f;
-  const uint32_t c = min((__float_as_uint(y) + noise) >> 20, 255u);
-  return max(c, x > 0.0f ? 1u : 0u);
+  const uint32_t t = __float_as_uint(__fmul_rn(__fmul_rn(x, inv), 0x1p-96f)) * 16u + noise;
+  return x > 0.0f ? max(t, 1u << 24) : t;
+}
+__device__ __forceinline__ uint32_t top_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+__device__ __forceinline__ float warp_max_nan(float x) {
+  float m;
+  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(x));
+  return m;
 }
 
-__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+// A lane's 8 of a block's 256 values: four at 4 * lane and four at 128 + 4 *
+// lane, so that every access of a warp to an fp32 array covers whole lines
+// (8 in a row, two 16-byte stores into each 32-byte sector: 4.4, not 6 TB/s).
+__device__ __forceinline__ int place(int lane, int i) { return lane * 4 + (i & 3) + (i >> 2) * 128; }
+__device__ __forceinline__ void load8(const float* p, int lane, float (&x)[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(p + lane * 4), b = *reinterpret_cast<const float4*>(p + 128 + lane * 4);
   x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
 }
-__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
-  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-  *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+__device__ __forceinline__ void store8(float* p, int lane, const float (&x)[8]) {
+  *reinterpret_cast<float4*>(p + lane * 4) = make_float4(x[0], x[1], x[2], x[3]);
+  *reinterpret_cast<float4*>(p + 128 + lane * 4) = make_float4(x[4], x[5], x[6], x[7]);
 }
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&x)[8]) {
-  const uint4 a = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, int lane, float (&x)[8]) {
+  const uint2 a = *reinterpret_cast<const uint2*>(p + lane * 4), b = *reinterpret_cast<const uint2*>(p + 128 + lane * 4);
+  const uint32_t w[4] = {a.x, a.y, b.x, b.y};
 #pragma unroll
   for (int q = 0; q < 4; ++q) x[2 * q] = bf16_lo(w[q]), x[2 * q + 1] = bf16_hi(w[q]);
 }
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&x)[8]) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3]), pack2_bf16(x[4], x[5]),
-                                            pack2_bf16(x[6], x[7]));
+__device__ __forceinline__ void store_words(__nv_bfloat16* p, int lane, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  *reinterpret_cast<uint2*>(p + lane * 4) = make_uint2(a, b);
+  *reinterpret_cast<uint2*>(p + 128 + lane * 4) = make_uint2(c, d);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, int lane, const float (&x)[8]) {
+  store_words(p, lane, pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3]), pack2_bf16(x[4], x[5]), pack2_bf16(x[6], x[7]));
+}
+__device__ __forceinline__ uint2 load_codes(const uint8_t* p, int lane) {
+  return make_uint2(*reinterpret_cast<const uint32_t*>(p + lane * 4), *reinterpret_cast<const uint32_t*>(p + 128 + lane * 4));
+}
+__device__ __forceinline__ void store_codes(uint8_t* p, int lane, uint32_t a, uint32_t b) {
+  *reinterpret_cast<uint32_t*>(p + lane * 4) = a;
+  *reinterpret_cast<uint32_t*>(p + 128 + lane * 4) = b;
 }
 __device__ __forceinline__ float as_f32(float x) { return x; }
 __device__ __forceinline__ float as_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ void put(float* p, float x) { *p = x; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
+__device__ __forceinline__ float sqrt_fast(float x) {
+  float y;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 struct StepConsts {
-  float keep_lr, step_size, rs2;  // lr, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+  float lr, step_size, rs2;  // lr, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
   uint32_t key;
 };
 
@@ -116,70 +176,63 @@ template <typename P, typename G, bool MASTER, int BITS>
 __device__ __forceinline__ void adamw_block(const AdamArgs& a, const StepConsts& k, P* param, const G* grad,
                                             float* master, int64_t at, int n, float keep, bool vec, int lane) {
   float p[8], g[8], m[8], v[8];
-  const int e0 = lane * 8;
-  const int mine = n - e0;  // real elements of this lane (any that is <= 0: none)
   if (vec && n >= 256) {
-    load8(grad + e0, g);
-    if constexpr (!MASTER) load8(param + e0, p);
+    load8(grad, lane, g);
+    if constexpr (!MASTER) load8(param, lane, p);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      g[i] = i < mine ? as_f32(grad[e0 + i]) : 0.0f;
-      if constexpr (!MASTER) p[i] = i < mine ? as_f32(param[e0 + i]) : 0.0f;
+      const int e = place(lane, i);
+      g[i] = e < n ? as_f32(grad[e]) : 0.0f;
+      if constexpr (!MASTER) p[i] = e < n ? as_f32(param[e]) : 0.0f;
     }
   }
-  if constexpr (MASTER) load8(master + e0, p);
+  if constexpr (MASTER) load8(master, lane, p);
 
   if constexpr (BITS == 32) {
-    load8(static_cast<const float*>(a.m) + at + e0, m);
-    load8(static_cast<const float*>(a.v) + at + e0, v);
+    load8(static_cast<const float*>(a.m) + at, lane, m);
+    load8(static_cast<const float*>(a.v) + at, lane, v);
   } else {
-    const uint2 cm = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.m) + at + e0);
-    const uint2 cv = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + at + e0);
+    const uint2 cm = load_codes(static_cast<const uint8_t*>(a.m) + at, lane);
+    const uint2 cv = load_codes(static_cast<const uint8_t*>(a.v) + at, lane);
     const float sm = a.m_scale[at >> 8], sv = a.v_scale[at >> 8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      m[i] = decode_m(((i < 4 ? cm.x : cm.y) >> (8 * (i & 3))) & 255u, sm);
-      v[i] = decode_v(((i < 4 ? cv.x : cv.y) >> (8 * (i & 3))) & 255u, sv);
-    }
+    decode_m(cm.x, sm, m, 0), decode_m(cm.y, sm, m, 4);
+    decode_v(cv.x, sv, v, 0), decode_v(cv.y, sv, v, 4);
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     m[i] = __fadd_rn(__fmul_rn(m[i], a.b1), __fmul_rn(g[i], a.c1));
     v[i] = __fadd_rn(__fmul_rn(v[i], a.b2), __fmul_rn(__fmul_rn(g[i], g[i]), a.c2));
-    const float down = fmaf(sqrtf(v[i]), k.rs2, a.eps);
-    p[i] = fmaf(p[i], keep, -k.step_size * (m[i] / down));
+    // the update alone goes through the approximate root and reciprocal
+    // (2 units of the last place; a v under 2^-126 counts as 0 beside eps)
+    p[i] = fmaf(p[i], keep, -k.step_size * (m[i] * rcp_fast(fmaf(sqrt_fast(v[i]), k.rs2, a.eps))));
   }
-  uint32_t kb = 0;
-  if constexpr (BITS == 8 || (!MASTER && sizeof(P) == 2)) kb = block_key(k.key, uint64_t(at) >> 8);
+  constexpr bool kStochastic = !MASTER && sizeof(P) == 2;
   uint32_t bits[8];
-  if constexpr (BITS == 8 || (!MASTER && sizeof(P) == 2)) {
+  if constexpr (BITS == 8 || kStochastic) {
+    const uint32_t kb = block_key(k.key, uint64_t(at) >> 8);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) bits[i] = element_bits(kb, e0 + i);
+    for (int i = 0; i < 8; ++i) bits[i] = element_bits(kb, place(lane, i));
   }
 
   if constexpr (BITS == 32) {
-    store8(static_cast<float*>(a.m) + at + e0, m);
-    store8(static_cast<float*>(a.v) + at + e0, v);
+    store8(static_cast<float*>(a.m) + at, lane, m);
+    store8(static_cast<float*>(a.v) + at, lane, v);
   } else {
-    uint32_t bm = 0, bv = 0;  // bit patterns order as the sizes do; a NaN is the largest
+    float sm = fabsf(m[0]), sv = v[0];  // of the block: a NaN if there is one
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      bm = max(bm, __float_as_uint(m[i]) & 0x7FFFFFFFu);
-      bv = max(bv, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    }
-    bm = max(__reduce_max_sync(0xffffffffu, bm), __float_as_uint(0x1p-100f));
-    bv = max(__reduce_max_sync(0xffffffffu, bv), __float_as_uint(0x1p-100f));
-    const float sm = __uint_as_float(bm), sv = __uint_as_float(bv);
+    for (int i = 1; i < 8; ++i) sm = max_nan(sm, fabsf(m[i])), sv = max_nan(sv, v[i]);
+    sm = max_nan(warp_max_nan(sm), 0x1p-100f), sv = max_nan(warp_max_nan(sv), 0x1p-100f);
     const float im = 1.0f / sm, iv = 1.0f / sv;
-    uint32_t cm[2] = {0, 0}, cv[2] = {0, 0};
+    uint32_t c[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      cm[i >> 2] |= encode_m(m[i], im, (bits[i] >> 16) << 4 | 8u) << (8 * (i & 3));
-      cv[i >> 2] |= encode_v(v[i], iv, (bits[i] & 0xFFFFu) << 4 | 8u) << (8 * (i & 3));
-    }
-    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.m) + at + e0) = make_uint2(cm[0], cm[1]);
-    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.v) + at + e0) = make_uint2(cv[0], cv[1]);
+    for (int i = 0; i < 8; ++i) c[i] = encode_m(m[i], im, __byte_perm(bits[i], 0x80u, 0x5324));
+    store_codes(static_cast<uint8_t*>(a.m) + at, lane, top_bytes(c[0], c[1], c[2], c[3]),
+                top_bytes(c[4], c[5], c[6], c[7]));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = encode_v(v[i], iv, __byte_perm(bits[i], 0x80u, 0x5104));
+    store_codes(static_cast<uint8_t*>(a.v) + at, lane, top_bytes(c[0], c[1], c[2], c[3]),
+                top_bytes(c[4], c[5], c[6], c[7]));
     if (lane == 0) {
       a.m_scale[at >> 8] = sm;
       a.v_scale[at >> 8] = sv;
@@ -188,41 +241,52 @@ __device__ __forceinline__ void adamw_block(const AdamArgs& a, const StepConsts&
   if constexpr (MASTER) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i >= mine) p[i] = 0.0f;  // the gap behind the tensor stays zero
-    store8(master + e0, p);
-  } else if constexpr (sizeof(P) == 2) {
-    // stochastic: 16 random bits below the last one kept (never through NaN or infinity)
+      if (place(lane, i) >= n) p[i] = 0.0f;  // the gap behind the tensor stays zero
+    store8(master, lane, p);
+  } else if constexpr (kStochastic) {
+    // 16 random bits below the last one kept (never through NaN or infinity)
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (fabsf(p[i]) < INFINITY)
-        p[i] = __uint_as_float((__float_as_uint(p[i]) + (more_bits(bits[i]) & 0xFFFFu)) & 0xFFFF0000u);
+      if (fabsf(p[i]) < INFINITY) p[i] = __uint_as_float(__float_as_uint(p[i]) + (more_bits(bits[i]) & 0xFFFFu));
   }
   if (vec && n >= 256) {
-    store8(param + e0, p);
+    if constexpr (kStochastic) {
+      uint32_t w[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        w[q] = __byte_perm(__float_as_uint(p[2 * q]), __float_as_uint(p[2 * q + 1]), 0x7632);
+      store_words(param, lane, w[0], w[1], w[2], w[3]);
+    } else {
+      store8(param, lane, p);
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < mine) put(param + e0 + i, p[i]);
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (kStochastic) p[i] = __uint_as_float(__float_as_uint(p[i]) & 0xFFFF0000u);
+      if (place(lane, i) < n) put(param + place(lane, i), p[i]);
+    }
   }
 }
 
+// Elements i0 .. i1 of a tensor, i0 a multiple of 256.
 template <typename P, typename G, bool MASTER, int BITS>
-__device__ __forceinline__ void adamw_chunk(const AdamArgs& a, const StepConsts& k, const mxg_adamw_tensor& t,
-                                            uint64_t g, int64_t i0) {
-  P* param = static_cast<P*>(t.param) + i0;
-  const G* grad = reinterpret_cast<const G*>(g) + i0;
-  float* master = MASTER ? a.master + t.master + i0 : nullptr;
-  const int n = int(min(t.numel - i0, int64_t(MXG_ADAMW_CHUNK)));
+__device__ __forceinline__ void adamw_run(const AdamArgs& a, const StepConsts& k, const mxg_adamw_tensor& t,
+                                          uint64_t g, int64_t i0, int64_t i1) {
+  P* param = static_cast<P*>(t.param);
+  const G* grad = reinterpret_cast<const G*>(g);
+  float* master = MASTER ? a.master + t.master : nullptr;
+  const int64_t offset = t.offset;
   const bool vec = ((reinterpret_cast<uintptr_t>(param) | reinterpret_cast<uintptr_t>(grad)) & 15) == 0;
-  const float keep = 1.0f - k.keep_lr * t.weight_decay;
+  const float keep = 1.0f - k.lr * t.weight_decay;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int b = warp * 256; b < n; b += kAdamThreads * 8)
-    adamw_block<P, G, MASTER, BITS>(a, k, param + b, grad + b, MASTER ? master + b : nullptr, t.offset + i0 + b, n - b,
-                                    keep, vec, lane);
+  for (int64_t b = i0 + warp * 256; b < i1; b += kAdamThreads * 8)
+    adamw_block<P, G, MASTER, BITS>(a, k, param + b, grad + b, MASTER ? master + b : nullptr, offset + b,
+                                    int(min(i1 - b, int64_t(256))), keep, vec, lane);
 }
 
+// A block takes a run of neighbouring chunks: their tensor is looked up once.
 template <int BITS>
-__global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const __grid_constant__ AdamArgs a) {
+__global__ void __launch_bounds__(kAdamThreads, BITS == 8 ? 3 : 4) adamw_kernel(const __grid_constant__ AdamArgs a) {
   __shared__ float s_bc[2];
   const int64_t t = *a.step + 1;
   // 1 - b^t = -expm1(t ln b): exact where b^t is close to 1
@@ -230,30 +294,32 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const __grid_consta
   if (threadIdx.x == 32) s_bc[1] = float(-expm1(double(t) * a.ln_b2));
   __syncthreads();
   StepConsts k;
-  k.keep_lr = a.lr_ptr ? *a.lr_ptr : a.lr;
-  k.step_size = k.keep_lr / s_bc[0];
+  k.lr = a.lr_ptr ? *a.lr_ptr : a.lr;
+  k.step_size = k.lr / s_bc[0];
   k.rs2 = 1.0f / sqrtf(s_bc[1]);
   k.key = step_key(a.seed_lo, a.seed_hi, uint32_t(t));
-  for (int64_t c = blockIdx.x; c < a.n_chunks; c += gridDim.x) {
-    const int ti = a.chunks[a.chunk0 + c];
+  int64_t c = blockIdx.x;
+  int ti = c < a.n_chunks ? a.chunks[a.chunk0 + c] : 0;
+  for (; c < a.n_chunks; c += gridDim.x) {
     const mxg_adamw_tensor& T = a.tensors[ti];
     const uint64_t tagged = a.grads[ti - a.tensor0];
+    const int64_t i0 = (a.chunk0 + c - T.first_chunk) * MXG_ADAMW_CHUNK, i1 = min(T.numel, i0 + MXG_ADAMW_CHUNK);
+    if (c + gridDim.x < a.n_chunks) ti = a.chunks[a.chunk0 + c + gridDim.x];
     if (tagged == 0) continue;
     const uint64_t g = tagged & ~kGradF32;
     const bool f32 = tagged & kGradF32;
-    const int64_t i0 = (a.chunk0 + c - T.first_chunk) * MXG_ADAMW_CHUNK;
     switch (T.kind) {
       case MXG_ADAMW_F32:
-        if (f32) adamw_chunk<float, float, false, BITS>(a, k, T, g, i0);
-        else adamw_chunk<float, __nv_bfloat16, false, BITS>(a, k, T, g, i0);
+        if (f32) adamw_run<float, float, false, BITS>(a, k, T, g, i0, i1);
+        else adamw_run<float, __nv_bfloat16, false, BITS>(a, k, T, g, i0, i1);
         break;
       case MXG_ADAMW_BF16_MASTER:
-        if (f32) adamw_chunk<__nv_bfloat16, float, true, BITS>(a, k, T, g, i0);
-        else adamw_chunk<__nv_bfloat16, __nv_bfloat16, true, BITS>(a, k, T, g, i0);
+        if (f32) adamw_run<__nv_bfloat16, float, true, BITS>(a, k, T, g, i0, i1);
+        else adamw_run<__nv_bfloat16, __nv_bfloat16, true, BITS>(a, k, T, g, i0, i1);
         break;
       default:
-        if (f32) adamw_chunk<__nv_bfloat16, float, false, BITS>(a, k, T, g, i0);
-        else adamw_chunk<__nv_bfloat16, __nv_bfloat16, false, BITS>(a, k, T, g, i0);
+        if (f32) adamw_run<__nv_bfloat16, float, false, BITS>(a, k, T, g, i0, i1);
+        else adamw_run<__nv_bfloat16, __nv_bfloat16, false, BITS>(a, k, T, g, i0, i1);
     }
   }
   // every block has read the step by the time the last one is done
@@ -267,22 +333,22 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const __grid_consta
   }
 }
 
-__global__ void __launch_bounds__(256) adamw_moments_kernel(const uint2* __restrict__ m, const uint2* __restrict__ v,
+// A warp takes blocks of 256.
+__global__ void __launch_bounds__(256) adamw_moments_kernel(const uint8_t* __restrict__ m,
+                                                            const uint8_t* __restrict__ v,
                                                             const float* __restrict__ m_scale,
-                                                            const float* __restrict__ v_scale, int64_t n,
+                                                            const float* __restrict__ v_scale, int64_t blocks,
                                                             float* __restrict__ m_out, float* __restrict__ v_out) {
-  const int64_t stride = int64_t(gridDim.x) * blockDim.x;
-  for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < n / 8; i += stride) {
-    const uint2 cm = __ldcs(m + i), cv = __ldcs(v + i);
-    const float sm = m_scale[i >> 5], sv = v_scale[i >> 5];
+  const int lane = threadIdx.x & 31;
+  const int64_t step = int64_t(gridDim.x) * 8;
+  for (int64_t b = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5); b < blocks; b += step) {
+    const uint2 cm = load_codes(m + b * 256, lane), cv = load_codes(v + b * 256, lane);
+    const float sm = m_scale[b], sv = v_scale[b];
     float x[8], y[8];
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      x[q] = decode_m(((q < 4 ? cm.x : cm.y) >> (8 * (q & 3))) & 255u, sm);
-      y[q] = decode_v(((q < 4 ? cv.x : cv.y) >> (8 * (q & 3))) & 255u, sv);
-    }
-    store8(m_out + i * 8, x);
-    store8(v_out + i * 8, y);
+    decode_m(cm.x, sm, x, 0), decode_m(cm.y, sm, x, 4);
+    decode_v(cv.x, sv, y, 0), decode_v(cv.y, sv, y, 4);
+    store8(m_out + b * 256, lane, x);
+    store8(v_out + b * 256, lane, y);
   }
 }
 
@@ -300,7 +366,7 @@ extern "C" int mxg_adamw_step(const mxg_adamw_tensor* tensors, int n_tensors, co
       !step || !done || (state_bits != 8 && state_bits != 32))
     return MXG_ERR_INVALID_ARGUMENT;
   if (state_bits == 8 && (!exp_avg_scale || !exp_avg_sq_scale)) return MXG_ERR_INVALID_ARGUMENT;
-  if (!(lr >= 0.0) || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0))
+  if (!(lr >= 0.0) || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps > 0.0))
     return MXG_ERR_INVALID_ARGUMENT;
   for (int i = 0; i < n_tensors; ++i) {
     if (chunk_begin[i] < 0 || chunk_begin[i + 1] < chunk_begin[i]) return MXG_ERR_INVALID_ARGUMENT;
@@ -348,9 +414,9 @@ extern "C" int mxg_adamw_moments(const void* exp_avg, const void* exp_avg_sq, co
     return MXG_ERR_MISALIGNED;
   int st = check_device();
   if (st) return st;
-  const int64_t want = (n / 8 + 255) / 256;
+  const int64_t blocks = n / MXG_ADAMW_BLOCK, want = (blocks + 7) / 8;
   adamw_moments_kernel<<<unsigned(std::min<int64_t>(want, int64_t(num_sms()) * 16)), 256, 0, (cudaStream_t)stream>>>(
-      static_cast<const uint2*>(exp_avg), static_cast<const uint2*>(exp_avg_sq), exp_avg_scale, exp_avg_sq_scale, n,
-      exp_avg_out, exp_avg_sq_out);
+      static_cast<const uint8_t*>(exp_avg), static_cast<const uint8_t*>(exp_avg_sq), exp_avg_scale, exp_avg_sq_scale,
+      blocks, exp_avg_out, exp_avg_sq_out);
   return cuda_status(cudaGetLastError());
 }

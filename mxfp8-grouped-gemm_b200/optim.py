@@ -55,8 +55,8 @@ class AdamW:
             raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
         if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
             raise ValueError(f"betas must lie in [0, 1), got {betas}")
-        if not eps >= 0.0:
-            raise ValueError(f"eps must not be negative, got {eps}")
+        if not eps > 0.0:
+            raise ValueError(f"eps must be positive, got {eps}")
         decay = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * len(params)
         if len(decay) != len(params):
             raise ValueError(f"{len(decay)} weight decays for {len(params)} tensors")
