@@ -12,6 +12,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "mxg.h"
 #include "mxg_device.cuh"
@@ -39,6 +40,30 @@ struct AdamArgs {
   uint32_t seed_lo, seed_hi;
   uint64_t grads[kAdamTensors];
 };
+
+// Two fp32 operations in one instruction, each rounded as a single one.
+struct Two {
+  uint64_t w;
+};
+__device__ __forceinline__ Two two(float a, float b) {
+  Two t;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(t.w) : "f"(a), "f"(b));
+  return t;
+}
+__device__ __forceinline__ Two both(float a) { return two(a, a); }
+__device__ __forceinline__ void split(Two t, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(t.w));
+}
+__device__ __forceinline__ Two mul(Two a, Two b) {
+  Two t;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(t.w) : "l"(a.w), "l"(b.w));
+  return t;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two t;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(t.w) : "l"(a.w), "l"(b.w), "l"(c.w));
+  return t;
+}
 
 // Random bits: 32x32 -> 64-bit products by odd constants, the halves xored,
 // two of them for each of (seed, step), block and element.  Means, spread and
@@ -92,21 +117,9 @@ __device__ __forceinline__ void decode_v(uint32_t codes, float scale, float (&x)
     for (int i = 0; i < 4; ++i) x[at + i] *= more;
   }
 }
-// The code as the top byte, sign apart; noise: 16 random bits, in bits 8 to 23.
-// (A NaN or infinity spills over, into a block whose scale is one too.)  The
-// two products are spelled out: nvcc 12.9 at -O3 drops what follows a plain
-// product by 2^-112 here and yields codes of 0.
-__device__ __forceinline__ uint32_t encode_m(float x, float inv, uint32_t noise) {
-  const uint32_t t = __float_as_uint(__fmul_rn(__fmul_rn(fabsf(x), inv), 0x1p-112f)) * 16u + noise;
-  return (t & 0x7FFFFFFFu) | (__float_as_uint(x) & 0x80000000u);
-}
-__device__ __forceinline__ uint32_t encode_v(float x, float inv, uint32_t noise) {
-  const uint32_t t = __float_as_uint(__fmul_rn(__fmul_rn(x, inv), 0x1p-96f)) * 16u + noise;
-  return x > 0.0f ? max(t, 1u << 24) : t;
-}
-__device__ __forceinline__ uint32_t top_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
-}
+// The code as the top byte, without a sign; noise: 16 random bits, in bits 8 to
+// 23.  (A NaN or infinity spills over, into a block whose scale is one too.)
+__device__ __forceinline__ uint32_t top_code(float x, uint32_t noise) { return __float_as_uint(x) * 16u + noise; }
 __device__ __forceinline__ float max_nan(float a, float b) {
   float m;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
@@ -121,34 +134,56 @@ __device__ __forceinline__ float warp_max_nan(float x) {
 // A lane's 8 of a block's 256 values: four at 4 * lane and four at 128 + 4 *
 // lane, so that every access of a warp to an fp32 array covers whole lines
 // (8 in a row, two 16-byte stores into each 32-byte sector: 4.4, not 6 TB/s).
+// They travel as words; pointers are to the lane's first value.
 __device__ __forceinline__ int place(int lane, int i) { return lane * 4 + (i & 3) + (i >> 2) * 128; }
-__device__ __forceinline__ void load8(const float* p, int lane, float (&x)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p + lane * 4), b = *reinterpret_cast<const float4*>(p + 128 + lane * 4);
-  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-}
-__device__ __forceinline__ void store8(float* p, int lane, const float (&x)[8]) {
-  *reinterpret_cast<float4*>(p + lane * 4) = make_float4(x[0], x[1], x[2], x[3]);
-  *reinterpret_cast<float4*>(p + 128 + lane * 4) = make_float4(x[4], x[5], x[6], x[7]);
-}
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, int lane, float (&x)[8]) {
-  const uint2 a = *reinterpret_cast<const uint2*>(p + lane * 4), b = *reinterpret_cast<const uint2*>(p + 128 + lane * 4);
-  const uint32_t w[4] = {a.x, a.y, b.x, b.y};
+template <typename T>
+struct Words {
+  static constexpr int N = 2 * sizeof(T);
+  uint32_t w[N];
+};
+template <typename T>
+__device__ __forceinline__ void fetch(const T* p, Words<T>& x) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) x[2 * q] = bf16_lo(w[q]), x[2 * q + 1] = bf16_hi(w[q]);
+  for (int h = 0; h < 2; ++h) {
+    const T* q = p + h * 128;
+    uint32_t* w = x.w + h * sizeof(T);
+    if constexpr (sizeof(T) == 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(q);
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else if constexpr (sizeof(T) == 2) {
+      const uint2 v = *reinterpret_cast<const uint2*>(q);
+      w[0] = v.x, w[1] = v.y;
+    } else {
+      w[0] = *reinterpret_cast<const uint32_t*>(q);
+    }
+  }
 }
-__device__ __forceinline__ void store_words(__nv_bfloat16* p, int lane, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  *reinterpret_cast<uint2*>(p + lane * 4) = make_uint2(a, b);
-  *reinterpret_cast<uint2*>(p + 128 + lane * 4) = make_uint2(c, d);
+template <typename T>
+__device__ __forceinline__ void keep_words(T* p, const Words<T>& x) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    T* q = p + h * 128;
+    const uint32_t* w = x.w + h * sizeof(T);
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(q) = make_uint4(w[0], w[1], w[2], w[3]);
+    else if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(q) = w[0];
+  }
 }
-__device__ __forceinline__ void store8(__nv_bfloat16* p, int lane, const float (&x)[8]) {
-  store_words(p, lane, pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3]), pack2_bf16(x[4], x[5]), pack2_bf16(x[6], x[7]));
+__device__ __forceinline__ void unpack(const Words<float>& x, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(x.w[i]);
 }
-__device__ __forceinline__ uint2 load_codes(const uint8_t* p, int lane) {
-  return make_uint2(*reinterpret_cast<const uint32_t*>(p + lane * 4), *reinterpret_cast<const uint32_t*>(p + 128 + lane * 4));
+__device__ __forceinline__ void unpack(const Words<__nv_bfloat16>& x, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[2 * i] = bf16_lo(x.w[i]), f[2 * i + 1] = bf16_hi(x.w[i]);
 }
-__device__ __forceinline__ void store_codes(uint8_t* p, int lane, uint32_t a, uint32_t b) {
-  *reinterpret_cast<uint32_t*>(p + lane * 4) = a;
-  *reinterpret_cast<uint32_t*>(p + 128 + lane * 4) = b;
+__device__ __forceinline__ void pack(const float (&f)[8], Words<float>& x) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x.w[i] = __float_as_uint(f[i]);
+}
+__device__ __forceinline__ void pack(const float (&f)[8], Words<__nv_bfloat16>& x) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x.w[i] = pack2_bf16(f[2 * i], f[2 * i + 1]);
 }
 __device__ __forceinline__ float as_f32(float x) { return x; }
 __device__ __forceinline__ float as_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -167,124 +202,176 @@ __device__ __forceinline__ float rcp_fast(float x) {
 }
 
 struct StepConsts {
-  float lr, step_size, rs2;  // lr, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+  float lr;
+  float rs2, eps;  // -1 / sqrt(1 - b2^t) and -eps, over lr / (1 - b1^t): m / (sqrt(v) rs2 + eps) is the step
   uint32_t key;
 };
 
-// 256 elements (n of them real) at element i of a tensor, `at` of the moments.
+// What a lane reads of a block: weights, gradients and moments.
 template <typename P, typename G, bool MASTER, int BITS>
-__device__ __forceinline__ void adamw_block(const AdamArgs& a, const StepConsts& k, P* param, const G* grad,
-                                            float* master, int64_t at, int n, float keep, bool vec, int lane) {
-  float p[8], g[8], m[8], v[8];
-  if (vec && n >= 256) {
-    load8(grad, lane, g);
-    if constexpr (!MASTER) load8(param, lane, p);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int e = place(lane, i);
-      g[i] = e < n ? as_f32(grad[e]) : 0.0f;
-      if constexpr (!MASTER) p[i] = e < n ? as_f32(param[e]) : 0.0f;
-    }
-  }
-  if constexpr (MASTER) load8(master, lane, p);
+struct Block {
+  using W = typename std::conditional<MASTER, float, P>::type;    // what takes the update
+  using S = typename std::conditional<BITS == 8, uint8_t, float>::type;
+  Words<W> p;
+  Words<G> g;
+  Words<S> m, v;
+  float sm, sv;                                                    // scales
+};
 
-  if constexpr (BITS == 32) {
-    load8(static_cast<const float*>(a.m) + at, lane, m);
-    load8(static_cast<const float*>(a.v) + at, lane, v);
-  } else {
-    const uint2 cm = load_codes(static_cast<const uint8_t*>(a.m) + at, lane);
-    const uint2 cv = load_codes(static_cast<const uint8_t*>(a.v) + at, lane);
-    const float sm = a.m_scale[at >> 8], sv = a.v_scale[at >> 8];
-    decode_m(cm.x, sm, m, 0), decode_m(cm.y, sm, m, 4);
-    decode_v(cv.x, sv, v, 0), decode_v(cv.y, sv, v, 4);
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    m[i] = __fadd_rn(__fmul_rn(m[i], a.b1), __fmul_rn(g[i], a.c1));
-    v[i] = __fadd_rn(__fmul_rn(v[i], a.b2), __fmul_rn(__fmul_rn(g[i], g[i]), a.c2));
-    // the update alone goes through the approximate root and reciprocal
-    // (2 units of the last place; a v under 2^-126 counts as 0 beside eps)
-    p[i] = fmaf(p[i], keep, -k.step_size * (m[i] * rcp_fast(fmaf(sqrt_fast(v[i]), k.rs2, a.eps))));
-  }
+// The update of one block, in place; block: its number in the moments.
+template <typename P, typename G, bool MASTER, int BITS>
+__device__ __forceinline__ void update(const AdamArgs& a, const StepConsts& k, float keep, uint64_t block, int lane,
+                                       Block<P, G, MASTER, BITS>& x) {
   constexpr bool kStochastic = !MASTER && sizeof(P) == 2;
-  uint32_t bits[8];
-  if constexpr (BITS == 8 || kStochastic) {
-    const uint32_t kb = block_key(k.key, uint64_t(at) >> 8);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) bits[i] = element_bits(kb, place(lane, i));
-  }
-
+  float p[8], g[8], m[8], v[8];
+  unpack(x.p, p);
+  unpack(x.g, g);
   if constexpr (BITS == 32) {
-    store8(static_cast<float*>(a.m) + at, lane, m);
-    store8(static_cast<float*>(a.v) + at, lane, v);
+    unpack(x.m, m);
+    unpack(x.v, v);
   } else {
-    float sm = fabsf(m[0]), sv = v[0];  // of the block: a NaN if there is one
-#pragma unroll
-    for (int i = 1; i < 8; ++i) sm = max_nan(sm, fabsf(m[i])), sv = max_nan(sv, v[i]);
-    sm = max_nan(warp_max_nan(sm), 0x1p-100f), sv = max_nan(warp_max_nan(sv), 0x1p-100f);
-    const float im = 1.0f / sm, iv = 1.0f / sv;
-    uint32_t c[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = encode_m(m[i], im, __byte_perm(bits[i], 0x80u, 0x5324));
-    store_codes(static_cast<uint8_t*>(a.m) + at, lane, top_bytes(c[0], c[1], c[2], c[3]),
-                top_bytes(c[4], c[5], c[6], c[7]));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = encode_v(v[i], iv, __byte_perm(bits[i], 0x80u, 0x5104));
-    store_codes(static_cast<uint8_t*>(a.v) + at, lane, top_bytes(c[0], c[1], c[2], c[3]),
-                top_bytes(c[4], c[5], c[6], c[7]));
-    if (lane == 0) {
-      a.m_scale[at >> 8] = sm;
-      a.v_scale[at >> 8] = sv;
-    }
+    decode_m(x.m.w[0], x.sm, m, 0), decode_m(x.m.w[1], x.sm, m, 4);
+    decode_v(x.v.w[0], x.sv, v, 0), decode_v(x.v.w[1], x.sv, v, 4);
   }
-  if constexpr (MASTER) {
+  // the update alone goes through the approximate root and reciprocal (2 units
+  // of the last place; a v under 2^-126 counts as 0 beside eps)
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (place(lane, i) >= n) p[i] = 0.0f;  // the gap behind the tensor stays zero
-    store8(master, lane, p);
-  } else if constexpr (kStochastic) {
-    // 16 random bits below the last one kept (never through NaN or infinity)
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (fabsf(p[i]) < INFINITY) p[i] = __uint_as_float(__float_as_uint(p[i]) + (more_bits(bits[i]) & 0xFFFFu));
+  for (int i = 0; i < 8; i += 2) {
+    const Two gg = two(g[i], g[i + 1]);
+    float d0, d1;
+    // (the sums one by one: a packed one is contracted with its product)
+    split(mul(gg, both(a.c1)), d0, d1);
+    split(mul(two(m[i], m[i + 1]), both(a.b1)), m[i], m[i + 1]);
+    m[i] = __fadd_rn(m[i], d0), m[i + 1] = __fadd_rn(m[i + 1], d1);
+    split(mul(mul(gg, gg), both(a.c2)), d0, d1);
+    split(mul(two(v[i], v[i + 1]), both(a.b2)), v[i], v[i + 1]);
+    v[i] = __fadd_rn(v[i], d0), v[i + 1] = __fadd_rn(v[i + 1], d1);
+    split(fma2(two(sqrt_fast(v[i]), sqrt_fast(v[i + 1])), both(k.rs2), both(k.eps)), d0, d1);
+    const Two by = mul(two(m[i], m[i + 1]), two(rcp_fast(d0), rcp_fast(d1)));
+    split(fma2(two(p[i], p[i + 1]), both(keep), by), p[i], p[i + 1]);
   }
-  if (vec && n >= 256) {
-    if constexpr (kStochastic) {
-      uint32_t w[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        w[q] = __byte_perm(__float_as_uint(p[2 * q]), __float_as_uint(p[2 * q + 1]), 0x7632);
-      store_words(param, lane, w[0], w[1], w[2], w[3]);
-    } else {
-      store8(param, lane, p);
-    }
+  float im = 0.0f, iv = 0.0f, rm[2], rv[2];
+  if constexpr (BITS == 32) {
+    pack(m, x.m);
+    pack(v, x.v);
   } else {
+    x.sm = fabsf(m[0]), x.sv = v[0];  // of the block: a NaN if there is one
+#pragma unroll
+    for (int i = 1; i < 8; ++i) x.sm = max_nan(x.sm, fabsf(m[i])), x.sv = max_nan(x.sv, v[i]);
+    x.sm = max_nan(warp_max_nan(x.sm), 0x1p-100f), x.sv = max_nan(warp_max_nan(x.sv), 0x1p-100f);
+    im = 1.0f / x.sm, iv = 1.0f / x.sv;
+  }
+  if constexpr (BITS == 8 || kStochastic) {
+    const uint32_t kb = block_key(k.key, block);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if constexpr (kStochastic) p[i] = __uint_as_float(__float_as_uint(p[i]) & 0xFFFF0000u);
-      if (place(lane, i) < n) put(param + place(lane, i), p[i]);
+      const uint32_t bits = element_bits(kb, place(lane, i));
+      if constexpr (BITS == 8) {
+        // relative to the scale, with the exponent field that makes bits 20 and up the code
+        if (i % 2 == 0) {
+          split(mul(mul(two(m[i], m[i + 1]), both(im)), both(0x1p-112f)), rm[0], rm[1]);
+          split(mul(mul(two(v[i], v[i + 1]), both(iv)), both(0x1p-96f)), rv[0], rv[1]);
+        }
+        // the new code enters at the top of its word
+        const uint32_t tm = top_code(rm[i % 2], __byte_perm(bits, 0x80u, 0x5324));
+        const uint32_t tv = top_code(rv[i % 2], __byte_perm(bits, 0x80u, 0x5104));
+        x.m.w[i >> 2] = __byte_perm(x.m.w[i >> 2], (tm & 0x7FFFFFFFu) | (__float_as_uint(m[i]) & 0x80000000u), 0x7321);
+        x.v.w[i >> 2] = __byte_perm(x.v.w[i >> 2], v[i] > 0.0f ? max(tv, 1u << 24) : tv, 0x7321);
+      }
+      // a bf16 weight without a copy: 16 random bits below the last one kept; the sum of a NaN's bits
+      // (0x7FFFFFFF, as arithmetic gives it) would pass over to a negative number
+      if constexpr (kStochastic) {
+        const int u = __float_as_int(p[i]);
+        const uint32_t r = uint32_t(max(int(uint32_t(u) + (more_bits(bits) & 0xFFFFu)), u));
+        x.p.w[i >> 1] = i & 1 ? __byte_perm(x.p.w[i >> 1], r, 0x7632) : r;
+      }
+    }
+  }
+  if constexpr (!kStochastic) pack(p, x.p);
+}
+
+// Elements i0 .. i0 + n of a tensor, i0 a multiple of 256, n at most a chunk.
+// Whole blocks of 16-byte-aligned tensors are read and written in vectors,
+// others element by element.  Addresses are those of the chunk, the same for
+// the whole block, plus a 32-bit offset.
+template <typename P, typename G, bool MASTER, int BITS>
+__device__ __forceinline__ void adamw_chunk(const AdamArgs& a, const StepConsts& k, const mxg_adamw_tensor& t,
+                                            uint64_t g, int64_t i0, int n) {
+  using B = Block<P, G, MASTER, BITS>;
+  using S = typename B::S;
+  constexpr uint32_t kStep = kAdamThreads * 8;
+  const uint32_t lane = threadIdx.x & 31;
+  const float keep = 1.0f - k.lr * t.weight_decay;
+  const int64_t at = t.offset + i0;
+  P* param = static_cast<P*>(t.param) + i0;
+  const G* grad = reinterpret_cast<const G*>(g) + i0;
+  typename B::W* weight;
+  if constexpr (MASTER) weight = a.master + t.master + i0;
+  else weight = param;
+  S *m = static_cast<S*>(a.m) + at, *v = static_cast<S*>(a.v) + at;
+  float *ms = a.m_scale + (at >> 8), *vs = a.v_scale + (at >> 8);
+  const uint64_t block = uint64_t(at) >> 8;
+  const bool vec = ((reinterpret_cast<uintptr_t>(param) | reinterpret_cast<uintptr_t>(grad)) & 15) == 0;
+  const uint32_t whole = vec ? uint32_t(n) & ~255u : 0;  // elements that go by in vectors
+
+  auto load = [&](uint32_t o, B& x) {  // o: of the lane's first value
+    fetch(weight + o, x.p);
+    fetch(grad + o, x.g);
+    fetch(m + o, x.m);
+    fetch(v + o, x.v);
+    if constexpr (BITS == 8) x.sm = ms[o >> 8], x.sv = vs[o >> 8];
+  };
+  uint32_t o = (threadIdx.x >> 5) * 256 + lane * 4;
+#pragma unroll 1
+  for (; o < uint32_t(n) + lane * 4; o += kStep) {
+    B x;
+    if (o < whole) {
+      load(o, x);
+    } else {
+      float p[8], f[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t e = o + (i & 3) + (i >> 2) * 128;
+        f[i] = e < n ? as_f32(grad[e]) : 0.0f;
+        p[i] = !MASTER && e < n ? as_f32(param[e]) : 0.0f;
+      }
+      pack(f, x.g);
+      if constexpr (MASTER) fetch(weight + o, x.p);
+      else pack(p, x.p);
+      fetch(m + o, x.m);
+      fetch(v + o, x.v);
+      if constexpr (BITS == 8) x.sm = ms[o >> 8], x.sv = vs[o >> 8];
+    }
+    update(a, k, keep, block + (o >> 8), lane, x);
+    keep_words(m + o, x.m);
+    keep_words(v + o, x.v);
+    if (BITS == 8 && lane == 0) ms[o >> 8] = x.sm, vs[o >> 8] = x.sv;
+    if (o < whole) {
+      keep_words(weight + o, x.p);
+      if constexpr (MASTER) {
+        float f[8];
+        Words<P> w;
+        unpack(x.p, f);
+        pack(f, w);
+        keep_words(param + o, w);
+      }
+    } else {
+      float p[8];
+      unpack(x.p, p);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t e = o + (i & 3) + (i >> 2) * 128;
+        if (e < n) put(param + e, p[i]);
+        else p[i] = 0.0f;  // the gap behind the tensor stays zero
+      }
+      if constexpr (MASTER) {
+        pack(p, x.p);
+        keep_words(weight + o, x.p);
+      }
     }
   }
 }
 
-// Elements i0 .. i1 of a tensor, i0 a multiple of 256.
-template <typename P, typename G, bool MASTER, int BITS>
-__device__ __forceinline__ void adamw_run(const AdamArgs& a, const StepConsts& k, const mxg_adamw_tensor& t,
-                                          uint64_t g, int64_t i0, int64_t i1) {
-  P* param = static_cast<P*>(t.param);
-  const G* grad = reinterpret_cast<const G*>(g);
-  float* master = MASTER ? a.master + t.master : nullptr;
-  const int64_t offset = t.offset;
-  const bool vec = ((reinterpret_cast<uintptr_t>(param) | reinterpret_cast<uintptr_t>(grad)) & 15) == 0;
-  const float keep = 1.0f - k.lr * t.weight_decay;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int64_t b = i0 + warp * 256; b < i1; b += kAdamThreads * 8)
-    adamw_block<P, G, MASTER, BITS>(a, k, param + b, grad + b, MASTER ? master + b : nullptr, offset + b,
-                                    int(min(i1 - b, int64_t(256))), keep, vec, lane);
-}
-
-// A block takes a run of neighbouring chunks: their tensor is looked up once.
 template <int BITS>
 __global__ void __launch_bounds__(kAdamThreads, BITS == 8 ? 3 : 4) adamw_kernel(const __grid_constant__ AdamArgs a) {
   __shared__ float s_bc[2];
@@ -295,31 +382,33 @@ __global__ void __launch_bounds__(kAdamThreads, BITS == 8 ? 3 : 4) adamw_kernel(
   __syncthreads();
   StepConsts k;
   k.lr = a.lr_ptr ? *a.lr_ptr : a.lr;
-  k.step_size = k.lr / s_bc[0];
-  k.rs2 = 1.0f / sqrtf(s_bc[1]);
+  const float size = -k.lr / s_bc[0];  // lr 0: both infinite, and the step 0
+  k.rs2 = 1.0f / (sqrtf(s_bc[1]) * size);
+  k.eps = a.eps / size;
   k.key = step_key(a.seed_lo, a.seed_hi, uint32_t(t));
   int64_t c = blockIdx.x;
   int ti = c < a.n_chunks ? a.chunks[a.chunk0 + c] : 0;
   for (; c < a.n_chunks; c += gridDim.x) {
     const mxg_adamw_tensor& T = a.tensors[ti];
     const uint64_t tagged = a.grads[ti - a.tensor0];
-    const int64_t i0 = (a.chunk0 + c - T.first_chunk) * MXG_ADAMW_CHUNK, i1 = min(T.numel, i0 + MXG_ADAMW_CHUNK);
+    const int64_t i0 = (a.chunk0 + c - T.first_chunk) * MXG_ADAMW_CHUNK;
+    const int n = int(min(T.numel - i0, int64_t(MXG_ADAMW_CHUNK)));
     if (c + gridDim.x < a.n_chunks) ti = a.chunks[a.chunk0 + c + gridDim.x];
     if (tagged == 0) continue;
     const uint64_t g = tagged & ~kGradF32;
     const bool f32 = tagged & kGradF32;
     switch (T.kind) {
       case MXG_ADAMW_F32:
-        if (f32) adamw_run<float, float, false, BITS>(a, k, T, g, i0, i1);
-        else adamw_run<float, __nv_bfloat16, false, BITS>(a, k, T, g, i0, i1);
+        if (f32) adamw_chunk<float, float, false, BITS>(a, k, T, g, i0, n);
+        else adamw_chunk<float, __nv_bfloat16, false, BITS>(a, k, T, g, i0, n);
         break;
       case MXG_ADAMW_BF16_MASTER:
-        if (f32) adamw_run<__nv_bfloat16, float, true, BITS>(a, k, T, g, i0, i1);
-        else adamw_run<__nv_bfloat16, __nv_bfloat16, true, BITS>(a, k, T, g, i0, i1);
+        if (f32) adamw_chunk<__nv_bfloat16, float, true, BITS>(a, k, T, g, i0, n);
+        else adamw_chunk<__nv_bfloat16, __nv_bfloat16, true, BITS>(a, k, T, g, i0, n);
         break;
       default:
-        if (f32) adamw_run<__nv_bfloat16, float, false, BITS>(a, k, T, g, i0, i1);
-        else adamw_run<__nv_bfloat16, __nv_bfloat16, false, BITS>(a, k, T, g, i0, i1);
+        if (f32) adamw_chunk<__nv_bfloat16, float, false, BITS>(a, k, T, g, i0, n);
+        else adamw_chunk<__nv_bfloat16, __nv_bfloat16, false, BITS>(a, k, T, g, i0, n);
     }
   }
   // every block has read the step by the time the last one is done
@@ -342,13 +431,18 @@ __global__ void __launch_bounds__(256) adamw_moments_kernel(const uint8_t* __res
   const int lane = threadIdx.x & 31;
   const int64_t step = int64_t(gridDim.x) * 8;
   for (int64_t b = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5); b < blocks; b += step) {
-    const uint2 cm = load_codes(m + b * 256, lane), cv = load_codes(v + b * 256, lane);
+    Words<uint8_t> cm, cv;
+    Words<float> out;
+    fetch(m + b * 256 + lane * 4, cm);
+    fetch(v + b * 256 + lane * 4, cv);
     const float sm = m_scale[b], sv = v_scale[b];
     float x[8], y[8];
-    decode_m(cm.x, sm, x, 0), decode_m(cm.y, sm, x, 4);
-    decode_v(cv.x, sv, y, 0), decode_v(cv.y, sv, y, 4);
-    store8(m_out + b * 256, lane, x);
-    store8(v_out + b * 256, lane, y);
+    decode_m(cm.w[0], sm, x, 0), decode_m(cm.w[1], sm, x, 4);
+    decode_v(cv.w[0], sv, y, 0), decode_v(cv.w[1], sv, y, 4);
+    pack(x, out);
+    keep_words(m_out + b * 256 + lane * 4, out);
+    pack(y, out);
+    keep_words(v_out + b * 256 + lane * 4, out);
   }
 }
 
