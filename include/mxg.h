@@ -337,7 +337,6 @@ MXG_API int mxg_router_topk_bwd(const void* logits, int64_t ld, int dtype, int64
  * rounded to nearest, or bf16 without one, rounded stochastically (to nearest
  * would lose every update under half a step). */
 #define MXG_ADAMW_BLOCK 256
-#define MXG_ADAMW_CHUNK 4096      /* elements a table entry covers */
 #define MXG_ADAMW_F32 0           /* kinds of weights */
 #define MXG_ADAMW_BF16_MASTER 1
 #define MXG_ADAMW_BF16 2
@@ -352,8 +351,9 @@ typedef struct mxg_adamw_tensor {
 } mxg_adamw_tensor;
 
 /* tensors [n_tensors] and chunks [n_chunks] are device arrays: chunks holds,
- * tensor after tensor, its index once for each MXG_ADAMW_CHUNK of its elements
- * (rounded up).  grads [n_tensors] is a HOST array of device addresses (0: no
+ * tensor after tensor, its index once for each `chunk` of its elements
+ * (rounded up; a multiple of 256, 4096 for a few million elements and more for
+ * hundreds of millions).  grads [n_tensors] is a HOST array of device addresses (0: no
  * gradient, the tensor and its moments are left as they are) and grad_dtypes
  * [n_tensors] the MXG_DTYPE_ of each (bf16 or f32); chunk_begin [n_tensors + 1]
  * a HOST array, the first entry of each tensor.  scales are [elements / 256]
@@ -364,7 +364,7 @@ typedef struct mxg_adamw_tensor {
  * device, zero between calls.  Calls on the same moments run one after the
  * other. */
 MXG_API int mxg_adamw_step(const mxg_adamw_tensor* tensors, int n_tensors, const int32_t* chunks,
-                           const int64_t* chunk_begin, const uint64_t* grads,
+                           const int64_t* chunk_begin, int chunk, const uint64_t* grads,
                            const int32_t* grad_dtypes, int state_bits, void* exp_avg,
                            void* exp_avg_sq, float* exp_avg_scale, float* exp_avg_sq_scale,
                            float* master, int64_t* step, int32_t* done, double lr,

@@ -33,7 +33,7 @@ EP_MAX_EXPERTS = 384
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 GROUP_MAX, GROUP_TOP2 = 0, 1
 ROUTER_MAX_TOPK, ROUTER_MAX_GROUPS = 32, 32
-ADAMW_BLOCK, ADAMW_CHUNK = 256, 4096
+ADAMW_BLOCK = 256
 ADAMW_F32, ADAMW_BF16_MASTER, ADAMW_BF16 = 0, 1, 2
 
 _c_i64, _c_int, _c_size, _vp = ctypes.c_int64, ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p
@@ -78,7 +78,7 @@ _PROTOS = {
                                  _c_int, _c_int, _c_f32, _vp, _vp, _vp]),
     "mxg_router_topk_bwd": (_c_int, [_vp, _c_i64, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_f32, _vp,
                                      _vp, _vp, _vp, _c_i64, _vp]),
-    "mxg_adamw_step": (_c_int, [_vp, _c_int, _vp, _vp, _vp, _vp, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_f64,
+    "mxg_adamw_step": (_c_int, [_vp, _c_int, _vp, _vp, _c_int, _vp, _vp, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_f64,
                                 _vp, _c_f64, _c_f64, _c_f64, _c_u64, _vp]),
     "mxg_adamw_moments": (_c_int, [_vp, _vp, _vp, _vp, _c_i64, _vp, _vp, _vp]),
     "mxg_swiglu": (_c_int, [_vp, _c_i64, _c_i64, _vp, _vp]),

@@ -1,8 +1,8 @@
 // One AdamW step over many tensors for sm_100a.
 //
-// The tensors are cut into chunks of MXG_ADAMW_CHUNK elements; every block takes
-// an equal run of the chunk table, a warp 256 elements at a time (8 a lane, the
-// block that shares one scale of the 8-bit moments).  Bound by HBM: every
+// The tensors are cut into chunks; a persistent grid walks their table, a warp
+// taking 256 elements at a time (8 a lane, the block that shares one scale of
+// the 8-bit moments).  Bound by HBM: every
 // array passes by once, in 16-byte accesses.
 //
 // The moments are rounded operation by operation (no fused multiply-adds), so
@@ -20,7 +20,9 @@
 
 namespace mxg {
 
-constexpr int kAdamThreads = 256;
+// One block an SM: its warps work on one run of memory (352 M weights, 8 bits: 868 us, 908 with two blocks of 512,
+// 948 with four of 256; 32 bits: 1627, 1630, 1645).
+constexpr int kAdamThreads = 1024;
 constexpr int kAdamTensors = 480;              // gradient addresses a launch carries (kernel arguments: 4 KB)
 constexpr uint64_t kGradF32 = uint64_t(1) << 63;
 
@@ -28,6 +30,7 @@ struct AdamArgs {
   const mxg_adamw_tensor* tensors;
   const int32_t* chunks;
   int64_t chunk0, n_chunks;
+  int chunk;
   int tensor0;
   bool last;                                   // this launch raises the step
   void *m, *v;
@@ -220,7 +223,7 @@ struct Block {
 
 // The update of one block, in place; block: its number in the moments.
 template <typename P, typename G, bool MASTER, int BITS>
-__device__ __forceinline__ void update(const AdamArgs& a, const StepConsts& k, float keep, uint64_t block, int lane,
+__device__ __forceinline__ void update(const AdamArgs& a, const StepConsts& k, float decay, uint64_t block, int lane,
                                        Block<P, G, MASTER, BITS>& x) {
   constexpr bool kStochastic = !MASTER && sizeof(P) == 2;
   float p[8], g[8], m[8], v[8];
@@ -247,8 +250,10 @@ __device__ __forceinline__ void update(const AdamArgs& a, const StepConsts& k, f
     split(mul(two(v[i], v[i + 1]), both(a.b2)), v[i], v[i + 1]);
     v[i] = __fadd_rn(v[i], d0), v[i + 1] = __fadd_rn(v[i + 1], d1);
     split(fma2(two(sqrt_fast(v[i]), sqrt_fast(v[i + 1])), both(k.rs2), both(k.eps)), d0, d1);
+    // the decay joins the update: one rounding of the weight's size
     const Two by = mul(two(m[i], m[i + 1]), two(rcp_fast(d0), rcp_fast(d1)));
-    split(fma2(two(p[i], p[i + 1]), both(keep), by), p[i], p[i + 1]);
+    split(fma2(two(p[i], p[i + 1]), both(decay), by), d0, d1);
+    p[i] += d0, p[i + 1] += d1;
   }
   float im = 0.0f, iv = 0.0f, rm[2], rv[2];
   if constexpr (BITS == 32) {
@@ -292,7 +297,10 @@ __device__ __forceinline__ void update(const AdamArgs& a, const StepConsts& k, f
 
 // Elements i0 .. i0 + n of a tensor, i0 a multiple of 256, n at most a chunk.
 // Whole blocks of 16-byte-aligned tensors are read and written in vectors,
-// others element by element.  Addresses are those of the chunk, the same for
+// others element by element.  With 8-bit moments the step is bound by
+// instructions, and registers are short: the next block is fetched to the L2
+// cache (352 M weights, blocks of 256 threads: 979 -> 935 us; through shared
+// memory instead 957, into registers 1265).  Addresses are those of the chunk, the same for
 // the whole block, plus a 32-bit offset.
 template <typename P, typename G, bool MASTER, int BITS>
 __device__ __forceinline__ void adamw_chunk(const AdamArgs& a, const StepConsts& k, const mxg_adamw_tensor& t,
@@ -301,7 +309,7 @@ __device__ __forceinline__ void adamw_chunk(const AdamArgs& a, const StepConsts&
   using S = typename B::S;
   constexpr uint32_t kStep = kAdamThreads * 8;
   const uint32_t lane = threadIdx.x & 31;
-  const float keep = 1.0f - k.lr * t.weight_decay;
+  const float decay = -k.lr * t.weight_decay;
   const int64_t at = t.offset + i0;
   P* param = static_cast<P*>(t.param) + i0;
   const G* grad = reinterpret_cast<const G*>(g) + i0;
@@ -321,12 +329,22 @@ __device__ __forceinline__ void adamw_chunk(const AdamArgs& a, const StepConsts&
     fetch(v + o, x.v);
     if constexpr (BITS == 8) x.sm = ms[o >> 8], x.sv = vs[o >> 8];
   };
+  // a line of 128 bytes a lane: gradients, weights, codes
+  constexpr uint32_t kG = 2 * sizeof(G), kW = 2 * sizeof(typename B::W);
+  auto prefetch = [&](uint32_t q) {
+    const char* from = lane < kG        ? reinterpret_cast<const char*>(grad + q) + lane * 128
+                       : lane < kG + kW ? reinterpret_cast<const char*>(weight + q) + (lane - kG) * 128
+                       : lane < kG + kW + 2 ? reinterpret_cast<const char*>(m + q) + (lane - kG - kW) * 128
+                                            : reinterpret_cast<const char*>(v + q) + (lane - kG - kW - 2) * 128;
+    if (lane < kG + kW + 4) asm volatile("prefetch.global.L2 [%0];" ::"l"(from));
+  };
   uint32_t o = (threadIdx.x >> 5) * 256 + lane * 4;
 #pragma unroll 1
   for (; o < uint32_t(n) + lane * 4; o += kStep) {
     B x;
     if (o < whole) {
       load(o, x);
+      if (BITS == 8 && o + kStep < whole) prefetch(o - lane * 4 + kStep);
     } else {
       float p[8], f[8];
 #pragma unroll
@@ -342,7 +360,7 @@ __device__ __forceinline__ void adamw_chunk(const AdamArgs& a, const StepConsts&
       fetch(v + o, x.v);
       if constexpr (BITS == 8) x.sm = ms[o >> 8], x.sv = vs[o >> 8];
     }
-    update(a, k, keep, block + (o >> 8), lane, x);
+    update(a, k, decay, block + (o >> 8), lane, x);
     keep_words(m + o, x.m);
     keep_words(v + o, x.v);
     if (BITS == 8 && lane == 0) ms[o >> 8] = x.sm, vs[o >> 8] = x.sv;
@@ -373,7 +391,7 @@ __device__ __forceinline__ void adamw_chunk(const AdamArgs& a, const StepConsts&
 }
 
 template <int BITS>
-__global__ void __launch_bounds__(kAdamThreads, BITS == 8 ? 3 : 4) adamw_kernel(const __grid_constant__ AdamArgs a) {
+__global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const __grid_constant__ AdamArgs a) {
   __shared__ float s_bc[2];
   const int64_t t = *a.step + 1;
   // 1 - b^t = -expm1(t ln b): exact where b^t is close to 1
@@ -391,8 +409,8 @@ __global__ void __launch_bounds__(kAdamThreads, BITS == 8 ? 3 : 4) adamw_kernel(
   for (; c < a.n_chunks; c += gridDim.x) {
     const mxg_adamw_tensor& T = a.tensors[ti];
     const uint64_t tagged = a.grads[ti - a.tensor0];
-    const int64_t i0 = (a.chunk0 + c - T.first_chunk) * MXG_ADAMW_CHUNK;
-    const int n = int(min(T.numel - i0, int64_t(MXG_ADAMW_CHUNK)));
+    const int64_t i0 = (a.chunk0 + c - T.first_chunk) * a.chunk;
+    const int n = int(min(T.numel - i0, int64_t(a.chunk)));
     if (c + gridDim.x < a.n_chunks) ti = a.chunks[a.chunk0 + c + gridDim.x];
     if (tagged == 0) continue;
     const uint64_t g = tagged & ~kGradF32;
@@ -451,7 +469,7 @@ __global__ void __launch_bounds__(256) adamw_moments_kernel(const uint8_t* __res
 using namespace mxg;
 
 extern "C" int mxg_adamw_step(const mxg_adamw_tensor* tensors, int n_tensors, const int32_t* chunks,
-                              const int64_t* chunk_begin, const uint64_t* grads, const int32_t* grad_dtypes,
+                              const int64_t* chunk_begin, int chunk, const uint64_t* grads, const int32_t* grad_dtypes,
                               int state_bits, void* exp_avg, void* exp_avg_sq, float* exp_avg_scale,
                               float* exp_avg_sq_scale, float* master, int64_t* step, int32_t* done, double lr,
                               const float* lr_ptr, double beta1, double beta2, double eps, uint64_t seed,
@@ -459,6 +477,7 @@ extern "C" int mxg_adamw_step(const mxg_adamw_tensor* tensors, int n_tensors, co
   if (n_tensors < 1 || !tensors || !chunks || !chunk_begin || !grads || !grad_dtypes || !exp_avg || !exp_avg_sq ||
       !step || !done || (state_bits != 8 && state_bits != 32))
     return MXG_ERR_INVALID_ARGUMENT;
+  if (chunk < MXG_ADAMW_BLOCK || chunk % MXG_ADAMW_BLOCK || chunk > (1 << 24)) return MXG_ERR_INVALID_ARGUMENT;
   if (state_bits == 8 && (!exp_avg_scale || !exp_avg_sq_scale)) return MXG_ERR_INVALID_ARGUMENT;
   if (!(lr >= 0.0) || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps > 0.0))
     return MXG_ERR_INVALID_ARGUMENT;
@@ -472,7 +491,7 @@ extern "C" int mxg_adamw_step(const mxg_adamw_tensor* tensors, int n_tensors, co
   int st = check_device();
   if (st) return st;
   AdamArgs a;
-  a.tensors = tensors, a.chunks = chunks;
+  a.tensors = tensors, a.chunks = chunks, a.chunk = chunk;
   a.m = exp_avg, a.v = exp_avg_sq, a.m_scale = exp_avg_scale, a.v_scale = exp_avg_sq_scale, a.master = master;
   a.step = step, a.done = done, a.lr_ptr = lr_ptr;
   a.lr = float(lr), a.b1 = float(beta1), a.c1 = float(1.0 - beta1), a.b2 = float(beta2), a.c2 = float(1.0 - beta2);

@@ -16,6 +16,9 @@ _ENTRY = np.dtype([("param", "<u8"), ("numel", "<i8"), ("offset", "<i8"), ("mast
                    ("kind", "<i4"), ("first_chunk", "<i8")])     # mxg_adamw_tensor
 
 
+_data_ptr, _get_device, _is_contiguous = torch.Tensor.data_ptr, torch.Tensor.get_device, torch.Tensor.is_contiguous
+
+
 def _padded(n: int) -> int:
     return -(-n // _lib.ADAMW_BLOCK) * _lib.ADAMW_BLOCK
 
@@ -75,6 +78,8 @@ class AdamW:
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("two of the params share memory")
         self.params, self.device = params, params[0].device
+        self._shapes, self._dtypes = [p.shape for p in params], [p.dtype for p in params]
+        self._on = {self.device.index}
         self.lr, self.betas, self.eps, self.weight_decay = lr, tuple(betas), eps, decay
         self.state_bits, self.master_weights, self.seed = state_bits, bool(master_weights), int(seed) & (2 ** 64 - 1)
         sizes = [_padded(p.numel()) for p in params]
@@ -101,7 +106,11 @@ class AdamW:
                         self.master[at:at + p.numel()].copy_(p.detach().reshape(-1))
         self._step = torch.zeros(1, dtype=torch.int64, device=dev)
         self._done = torch.zeros(1, dtype=torch.int32, device=dev)
-        chunks = [-(-p.numel() // _lib.ADAMW_CHUNK) for p in params]
+        # What a thread block takes at a time: about 128 shares, long runs where there is much.  us of a bf16 step
+        # with 32 / 8 bits at 4096, 8192, 32768: 1 M values 6.7 / 8.6, 6.7 / 7.9, 13.8 / 15.7; 64 M 330 / 289,
+        # 339 / 219, 337 / 185.
+        self._chunk = min(32768, max(4096, 1 << max(0, (self.offsets[-1] // 128).bit_length() - 1)))
+        chunks = [-(-p.numel() // self._chunk) for p in params]
         self._chunk_begin = np.concatenate([[0], np.cumsum(chunks)]).astype(np.int64)
         table = np.repeat(np.arange(len(params), dtype=np.int32), chunks)
         self._chunks = torch.from_numpy(table if table.size else np.zeros(1, np.int32)).to(dev)
@@ -109,6 +118,10 @@ class AdamW:
 
     def _lay_out(self):
         """The device table of the tensors (again when one has moved)."""
+        for i, (p, shape) in enumerate(zip(self.params, self._shapes)):
+            if p.shape != shape or p.dtype != self._dtypes[i] or p.device != self.device or not p.is_contiguous():
+                raise ValueError(f"params[{i}] is no longer a contiguous {tuple(shape)} {self._dtypes[i]} tensor on "
+                                 f"{self.device}")
         self._at = [p.data_ptr() for p in self.params]
         t = np.zeros(len(self.params), _ENTRY)
         t["param"], t["numel"] = self._at, [p.numel() for p in self.params]
@@ -135,33 +148,47 @@ class AdamW:
             lr, lr_ptr = 0.0, lr.data_ptr()
         elif not 0.0 <= lr < float("inf"):
             raise ValueError(f"lr must not be negative, got {lr}")
-        ptrs = np.zeros(len(params), np.uint64)
-        kinds = np.zeros(len(params), np.int32)
-        held = []                                  # contiguous copies, until the launch
-        for i, (p, g) in enumerate(zip(params, grads)):
-            if g is None:
-                continue
-            if g.dtype not in _GRAD:
-                raise TypeError(f"grads[{i}] must be bf16 or fp32, got {g.dtype}")
-            if g.shape != p.shape or g.device != self.device:
-                raise ValueError(f"grads[{i}] is {tuple(g.shape)} on {g.device}, expected {tuple(p.shape)} on "
-                                 f"{self.device}")
-            if not g.is_contiguous():
-                g = g.contiguous()
-                held.append(g)
-            ptrs[i], kinds[i] = g.data_ptr(), _GRAD[g.dtype]
-        if [p.data_ptr() for p in params] != self._at or self.weight_decay != self._laid_out:
+        held = None                                # contiguous copies, until the launch
+        # all at once where every gradient is as it should be
+        types = self._types(grads)
+        if (None in types or [g.shape for g in grads] != self._shapes
+                or set(map(_get_device, grads)) != self._on or not all(map(_is_contiguous, grads))):
+            grads = held = self._checked(grads)
+            types = self._types(grads)
+        kinds = np.array([t or 0 for t in types] if held else types, np.int32)
+        ptrs = np.array([0 if g is None else g.data_ptr() for g in grads] if held else list(map(_data_ptr, grads)),
+                        np.uint64)
+        if list(map(_data_ptr, params)) != self._at or self.weight_decay != self._laid_out:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("a tensor moved since the last step: take one step before the capture")
             self._lay_out()
         _lib.launch("mxg_adamw_step", self.device, self._table.data_ptr(), len(params), self._chunks.data_ptr(),
-                    self._chunk_begin.ctypes.data, ptrs.ctypes.data, kinds.ctypes.data, self.state_bits,
+                    self._chunk_begin.ctypes.data, self._chunk, ptrs.ctypes.data, kinds.ctypes.data, self.state_bits,
                     self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), _lib.ptr(self.exp_avg_scale),
                     _lib.ptr(self.exp_avg_sq_scale), _lib.ptr(self.master), self._step.data_ptr(),
                     self._done.data_ptr(), lr, lr_ptr, self.betas[0], self.betas[1], self.eps, self.seed)
+        del held
         tracked = [p for p in params if p.requires_grad]
         if tracked:                                # autograd sees the change in place
             torch.autograd.graph.increment_version(tracked)
+
+    @staticmethod
+    def _types(grads):
+        return [None if g is None else _GRAD.get(g.dtype) for g in grads]
+
+    def _checked(self, grads):
+        """The gradients one by one: refusals, and contiguous copies where needed."""
+        out = []
+        for i, (g, shape) in enumerate(zip(grads, self._shapes)):
+            if g is not None:
+                if g.dtype not in _GRAD:
+                    raise TypeError(f"grads[{i}] must be bf16 or fp32, got {g.dtype}")
+                if g.shape != shape or g.device != self.device:
+                    raise ValueError(f"grads[{i}] is {tuple(g.shape)} on {g.device}, expected {tuple(shape)} on "
+                                     f"{self.device}")
+                g = g.contiguous()
+            out.append(g)
+        return out
 
     def moments(self):
         """(exp_avg, exp_avg_sq) as flat fp32 arrays: the state itself with 32

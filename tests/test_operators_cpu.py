@@ -93,11 +93,12 @@ def test_adamw_abi_refuses_bad_arguments(mxg):
     begin, grads, kinds = np.zeros(2, np.int64), np.array([16], np.uint64), np.array([1], np.int32)
 
     def call(n=1, bits=32, m=16, ms=None, lr=1e-3, b1=0.9, b2=0.99, eps=1e-8, grads=grads, kinds=kinds, begin=begin,
-             step=16):
-        return L.mxg_adamw_step(16, n, 16, begin.ctypes.data, grads.ctypes.data, kinds.ctypes.data, bits, m, 16, ms,
+             step=16, chunk=4096):
+        return L.mxg_adamw_step(16, n, 16, begin.ctypes.data, chunk, grads.ctypes.data, kinds.ctypes.data, bits, m, 16, ms,
                                 ms, None, step, 16, lr, None, b1, b2, eps, 0, None)
     assert call(n=0) == 1 and call(bits=16) == 1 and call(m=None) == 1 and call(step=None) == 1
     assert call(bits=8) == 1                                     # no scales
+    assert call(chunk=0) == 1 and call(chunk=4000) == 1
     assert call(lr=-1.0) == 1 and call(b1=1.0) == 1 and call(b2=-0.1) == 1 and call(eps=float("nan")) == 1
     assert call(kinds=np.array([2], np.int32)) == 1
     assert call(grads=np.array([18], np.uint64)) == 3 and call(m=24) == 3
@@ -114,7 +115,7 @@ def test_tensor_table_matches_the_header(mxg):
     assert [e.fields[n][1] for n in ("param", "numel", "offset", "master", "decay", "kind", "first_chunk")] == \
         [0, 8, 16, 24, 32, 36, 40]
     text = open(mxg._lib.HEADER_PATH).read()
-    for name, value in (("MXG_ADAMW_BLOCK", 256), ("MXG_ADAMW_CHUNK", 4096), ("MXG_ROUTER_MAX_TOPK", 32),
+    for name, value in (("MXG_ADAMW_BLOCK", 256), ("MXG_ROUTER_MAX_TOPK", 32),
                         ("MXG_ROUTER_MAX_GROUPS", 32), ("MXG_EP_MAX_EXPERTS", 384)):
         assert f"#define {name} {value}" in text
         assert getattr(mxg._lib, name[4:]) == value
