@@ -267,7 +267,8 @@ MXG_API int mxg_ep_combine_rows(const void* rows, int64_t n_rows, const int32_t*
  * 1).  A negative position has no row: its dweights are 0.  One that is >=
  * n_rows is skipped too and sets the device error word to
  * MXG_ERR_INVALID_ARGUMENT.  slot_pos names a position at most once, as
- * mxg_ep_route gives it; rows of drows that it does not name become zero. */
+ * mxg_ep_route gives it (one named twice sets the error word too, and each
+ * element of its row of drows is that of either); rows that it does not name become zero. */
 MXG_API int mxg_ep_combine_bwd(const void* dout, const void* rows, const int32_t* slot_pos,
                                const float* weights, int64_t n_tokens, int topk, int64_t hidden,
                                int64_t n_rows, void* drows, float* dweights, void* stream);
@@ -305,20 +306,31 @@ MXG_API int mxg_swiglu_bwd(const void* gu, const void* dh, int64_t rows, int64_t
 #define MXG_GROUP_TOP2 1
 #define MXG_ROUTER_MAX_TOPK 32
 #define MXG_ROUTER_MAX_GROUPS 32
-MXG_API int mxg_router_topk(const void* logits, int64_t ld, int dtype, int64_t n_tokens,
-                            int num_experts, int topk, int score, const float* bias, int groups,
-                            int topk_groups, int group_score, int renormalize, float scale,
-                            float* weights, int32_t* ids, void* stream);
+typedef struct mxg_router_args {
+  const void* logits;
+  const float* bias;              /* or null                                  */
+  float* weights;                 /* [n_tokens, topk]                         */
+  int32_t* ids;                   /* [n_tokens, topk]                         */
+  const float* dweights;          /* [n_tokens, topk]     mxg_router_topk_bwd */
+  void* dlogits;                  /* like logits          mxg_router_topk_bwd */
+  int64_t n_tokens;
+  int64_t ld;                     /* row stride of logits                     */
+  int64_t ld_out;                 /* row stride of dlogits                    */
+  int32_t dtype;                  /* MXG_DTYPE_ of logits and dlogits         */
+  int32_t num_experts, topk;
+  int32_t score;                  /* MXG_SCORE_                               */
+  int32_t groups, topk_groups, group_score;
+  int32_t renormalize;
+  float scale;
+  int32_t reserved;
+} mxg_router_args;
+MXG_API int mxg_router_topk(const mxg_router_args* args, void* stream);
 
-/* Gradient of the logits (same dtype, row stride ld_out; every element is
- * written) from dweights [n_tokens, topk], and the weights and ids that
- * mxg_router_topk gave.  The choice itself has no gradient.  An id out of
- * range is skipped and sets the device error word; one named twice gets the
- * sum. */
-MXG_API int mxg_router_topk_bwd(const void* logits, int64_t ld, int dtype, int64_t n_tokens,
-                                int num_experts, int topk, int score, int renormalize, float scale,
-                                const float* weights, const int32_t* ids, const float* dweights,
-                                void* dlogits, int64_t ld_out, void* stream);
+/* Gradient of the logits (every element of dlogits is written) from dweights,
+ * and the weights and ids that mxg_router_topk gave (bias and groups are not
+ * read).  The choice itself has no gradient.  An id out of range is skipped and
+ * sets the device error word; one named twice gets the sum. */
+MXG_API int mxg_router_topk_bwd(const mxg_router_args* args, void* stream);
 
 /* ---- AdamW over many tensors in one launch ----
  * Moments are flat arrays in which tensor i starts at element offset[i], a
@@ -353,23 +365,33 @@ typedef struct mxg_adamw_tensor {
 /* tensors [n_tensors] and chunks [n_chunks] are device arrays: chunks holds,
  * tensor after tensor, its index once for each `chunk` of its elements
  * (rounded up; a multiple of 256, 4096 for a few million elements and more for
- * hundreds of millions).  grads [n_tensors] is a HOST array of device addresses (0: no
- * gradient, the tensor and its moments are left as they are) and grad_dtypes
- * [n_tensors] the MXG_DTYPE_ of each (bf16 or f32); chunk_begin [n_tensors + 1]
- * a HOST array, the first entry of each tensor.  scales are [elements / 256]
- * f32, null with 32 bits; master may be null without such tensors.  step is one
- * int64 on the device, the steps taken so far: it is read and then raised by
- * one, so a captured launch counts on when it is replayed.  lr_ptr, when not
- * null, is one f32 on the device that replaces lr.  done is one int32 on the
+ * hundreds of millions).  chunk_begin [n_tensors + 1] is a HOST array, the first
+ * entry of each tensor; grads [n_tensors] a HOST array of device addresses (0:
+ * no gradient, the tensor and its moments are left as they are) and grad_dtypes
+ * [n_tensors] the MXG_DTYPE_ of each (bf16 or f32).  step is one int64 on the
+ * device, the steps taken so far: it is read and then raised by one, so a
+ * captured launch counts on when it is replayed.  done is one int32 on the
  * device, zero between calls.  Calls on the same moments run one after the
  * other. */
-MXG_API int mxg_adamw_step(const mxg_adamw_tensor* tensors, int n_tensors, const int32_t* chunks,
-                           const int64_t* chunk_begin, int chunk, const uint64_t* grads,
-                           const int32_t* grad_dtypes, int state_bits, void* exp_avg,
-                           void* exp_avg_sq, float* exp_avg_scale, float* exp_avg_sq_scale,
-                           float* master, int64_t* step, int32_t* done, double lr,
-                           const float* lr_ptr, double beta1, double beta2, double eps,
-                           uint64_t seed, void* stream);
+typedef struct mxg_adamw_args {
+  const mxg_adamw_tensor* tensors;
+  const int32_t* chunks;
+  const int64_t* chunk_begin;
+  const uint64_t* grads;
+  const int32_t* grad_dtypes;
+  void* exp_avg;                  /* f32, or a byte a value                   */
+  void* exp_avg_sq;
+  float* exp_avg_scale;           /* one a block of 256; null with 32 bits    */
+  float* exp_avg_sq_scale;
+  float* master;                  /* null without such tensors                */
+  int64_t* step;
+  int32_t* done;
+  const float* lr_ptr;            /* one f32 on the device, or null: lr       */
+  double lr, beta1, beta2, eps;
+  uint64_t seed;
+  int32_t n_tensors, chunk, state_bits, reserved;
+} mxg_adamw_args;
+MXG_API int mxg_adamw_step(const mxg_adamw_args* args, void* stream);
 
 /* The f32 values of 8-bit moments (n elements, a multiple of 256). */
 MXG_API int mxg_adamw_moments(const void* exp_avg, const void* exp_avg_sq, const float* exp_avg_scale,

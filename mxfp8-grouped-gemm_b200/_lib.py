@@ -8,6 +8,7 @@ from __future__ import annotations
 import ctypes
 import os
 import re
+import struct
 import threading
 
 import torch
@@ -37,7 +38,6 @@ ADAMW_BLOCK = 256
 ADAMW_F32, ADAMW_BF16_MASTER, ADAMW_BF16 = 0, 1, 2
 
 _c_i64, _c_int, _c_size, _vp = ctypes.c_int64, ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p
-_c_f32, _c_f64, _c_u64 = ctypes.c_float, ctypes.c_double, ctypes.c_uint64
 _i32p = ctypes.POINTER(ctypes.c_int32)
 
 _PROTOS = {
@@ -74,12 +74,9 @@ _PROTOS = {
     "mxg_ep_combine": (_c_int, [_vp, _vp, _vp, _c_i64, _c_int, _c_i64, _vp, _vp]),
     "mxg_ep_combine_rows": (_c_int, [_vp, _c_i64, _vp, _vp, _c_i64, _c_int, _c_i64, _vp, _vp]),
     "mxg_ep_combine_bwd": (_c_int, [_vp, _vp, _vp, _vp, _c_i64, _c_int, _c_i64, _c_i64, _vp, _vp, _vp]),
-    "mxg_router_topk": (_c_int, [_vp, _c_i64, _c_int, _c_i64, _c_int, _c_int, _c_int, _vp, _c_int, _c_int,
-                                 _c_int, _c_int, _c_f32, _vp, _vp, _vp]),
-    "mxg_router_topk_bwd": (_c_int, [_vp, _c_i64, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_f32, _vp,
-                                     _vp, _vp, _vp, _c_i64, _vp]),
-    "mxg_adamw_step": (_c_int, [_vp, _c_int, _vp, _vp, _c_int, _vp, _vp, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_f64,
-                                _vp, _c_f64, _c_f64, _c_f64, _c_u64, _vp]),
+    "mxg_router_topk": (_c_int, [ctypes.c_char_p, _vp]),
+    "mxg_router_topk_bwd": (_c_int, [ctypes.c_char_p, _vp]),
+    "mxg_adamw_step": (_c_int, [ctypes.c_char_p, _vp]),
     "mxg_adamw_moments": (_c_int, [_vp, _vp, _vp, _vp, _c_i64, _vp, _vp, _vp]),
     "mxg_swiglu": (_c_int, [_vp, _c_i64, _c_i64, _vp, _vp]),
     "mxg_swiglu_bwd": (_c_int, [_vp, _vp, _c_i64, _c_i64, _vp, _vp]),
@@ -110,6 +107,11 @@ _PROTOS = {
 
 _lock = threading.Lock()
 _lib = None
+
+
+# mxg_router_args and mxg_adamw_args as bytes: one argument to convert instead of about 20
+router_args = struct.Struct("@6P3q8ifi").pack
+adamw_args = struct.Struct("@13P4dQ4i").pack
 
 
 class MxgError(RuntimeError):

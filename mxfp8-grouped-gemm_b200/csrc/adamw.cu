@@ -468,18 +468,19 @@ __global__ void __launch_bounds__(256) adamw_moments_kernel(const uint8_t* __res
 
 using namespace mxg;
 
-extern "C" int mxg_adamw_step(const mxg_adamw_tensor* tensors, int n_tensors, const int32_t* chunks,
-                              const int64_t* chunk_begin, int chunk, const uint64_t* grads, const int32_t* grad_dtypes,
-                              int state_bits, void* exp_avg, void* exp_avg_sq, float* exp_avg_scale,
-                              float* exp_avg_sq_scale, float* master, int64_t* step, int32_t* done, double lr,
-                              const float* lr_ptr, double beta1, double beta2, double eps, uint64_t seed,
-                              void* stream) {
-  if (n_tensors < 1 || !tensors || !chunks || !chunk_begin || !grads || !grad_dtypes || !exp_avg || !exp_avg_sq ||
-      !step || !done || (state_bits != 8 && state_bits != 32))
+extern "C" int mxg_adamw_step(const mxg_adamw_args* args, void* stream) {
+  if (!args) return MXG_ERR_INVALID_ARGUMENT;
+  const mxg_adamw_args& r = *args;
+  const int n_tensors = r.n_tensors, state_bits = r.state_bits;
+  const int64_t* chunk_begin = r.chunk_begin;
+  const uint64_t* grads = r.grads;
+  const int32_t* grad_dtypes = r.grad_dtypes;
+  if (n_tensors < 1 || !r.tensors || !r.chunks || !chunk_begin || !grads || !grad_dtypes || !r.exp_avg ||
+      !r.exp_avg_sq || !r.step || !r.done || (state_bits != 8 && state_bits != 32))
     return MXG_ERR_INVALID_ARGUMENT;
-  if (chunk < MXG_ADAMW_BLOCK || chunk % MXG_ADAMW_BLOCK || chunk > (1 << 24)) return MXG_ERR_INVALID_ARGUMENT;
-  if (state_bits == 8 && (!exp_avg_scale || !exp_avg_sq_scale)) return MXG_ERR_INVALID_ARGUMENT;
-  if (!(lr >= 0.0) || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps > 0.0))
+  if (r.chunk < MXG_ADAMW_BLOCK || r.chunk % MXG_ADAMW_BLOCK || r.chunk > (1 << 24)) return MXG_ERR_INVALID_ARGUMENT;
+  if (state_bits == 8 && (!r.exp_avg_scale || !r.exp_avg_sq_scale)) return MXG_ERR_INVALID_ARGUMENT;
+  if (!(r.lr >= 0.0) || !(r.beta1 >= 0.0 && r.beta1 < 1.0) || !(r.beta2 >= 0.0 && r.beta2 < 1.0) || !(r.eps > 0.0))
     return MXG_ERR_INVALID_ARGUMENT;
   for (int i = 0; i < n_tensors; ++i) {
     if (chunk_begin[i] < 0 || chunk_begin[i + 1] < chunk_begin[i]) return MXG_ERR_INVALID_ARGUMENT;
@@ -487,17 +488,17 @@ extern "C" int mxg_adamw_step(const mxg_adamw_tensor* tensors, int n_tensors, co
       return MXG_ERR_INVALID_ARGUMENT;
     if (grads[i] & kGradF32 || grads[i] % (grad_dtypes[i] == MXG_DTYPE_F32 ? 4 : 2)) return MXG_ERR_MISALIGNED;
   }
-  if (!aligned16(exp_avg) || !aligned16(exp_avg_sq) || !aligned16(master)) return MXG_ERR_MISALIGNED;
+  if (!aligned16(r.exp_avg) || !aligned16(r.exp_avg_sq) || !aligned16(r.master)) return MXG_ERR_MISALIGNED;
   int st = check_device();
   if (st) return st;
   AdamArgs a;
-  a.tensors = tensors, a.chunks = chunks, a.chunk = chunk;
-  a.m = exp_avg, a.v = exp_avg_sq, a.m_scale = exp_avg_scale, a.v_scale = exp_avg_sq_scale, a.master = master;
-  a.step = step, a.done = done, a.lr_ptr = lr_ptr;
-  a.lr = float(lr), a.b1 = float(beta1), a.c1 = float(1.0 - beta1), a.b2 = float(beta2), a.c2 = float(1.0 - beta2);
-  a.eps = float(eps);
-  a.ln_b1 = std::log(beta1), a.ln_b2 = std::log(beta2);
-  a.seed_lo = uint32_t(seed), a.seed_hi = uint32_t(seed >> 32);
+  a.tensors = r.tensors, a.chunks = r.chunks, a.chunk = r.chunk;
+  a.m = r.exp_avg, a.v = r.exp_avg_sq, a.m_scale = r.exp_avg_scale, a.v_scale = r.exp_avg_sq_scale, a.master = r.master;
+  a.step = r.step, a.done = r.done, a.lr_ptr = r.lr_ptr;
+  a.lr = float(r.lr), a.b1 = float(r.beta1), a.c1 = float(1.0 - r.beta1);
+  a.b2 = float(r.beta2), a.c2 = float(1.0 - r.beta2), a.eps = float(r.eps);
+  a.ln_b1 = std::log(r.beta1), a.ln_b2 = std::log(r.beta2);
+  a.seed_lo = uint32_t(r.seed), a.seed_hi = uint32_t(r.seed >> 32);
   int per_sm = 0;
   auto* kernel = state_bits == 8 ? adamw_kernel<8> : adamw_kernel<32>;
   if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kAdamThreads, 0) != cudaSuccess || per_sm < 1)

@@ -236,14 +236,16 @@ constexpr int kFillRows = 32768;
 
 __device__ __forceinline__ void zero_unnamed_rows(const int32_t* __restrict__ inv, int64_t n, int64_t first,
                                                   int64_t n_rows, int64_t vecs, uint4* __restrict__ rows,
-                                                  uint32_t* named) {
+                                                  uint32_t* named, int* err) {
   const int count = int(min(int64_t(kFillRows), n_rows - first));
   for (int i = threadIdx.x; i < kFillRows / 32; i += blockDim.x) named[i] = 0;
   __syncthreads();
 #pragma unroll 8
   for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
     const int64_t p = inv[i] - first;
-    if (p >= 0 && p < count) atomicOr(&named[p >> 5], 1u << (p & 31));
+    if (p < 0 || p >= count) continue;
+    const uint32_t bit = 1u << (p & 31);  // a row named twice has no single gradient
+    if (atomicOr(&named[p >> 5], bit) & bit) atomicCAS(err, 0, MXG_ERR_INVALID_ARGUMENT);
   }
   __syncthreads();
   for (int i = 0; i < (count + 31) / 32; ++i) {
@@ -268,7 +270,7 @@ __global__ void __launch_bounds__(256) combine_bwd_kernel(const __nv_bfloat16* _
   __shared__ uint32_t named[kFillRows / 32];
   if (int(blockIdx.x) < fill_blocks) {
     zero_unnamed_rows(inv, n_tokens * topk, int64_t(blockIdx.x) * kFillRows, n_rows, hidden / 8,
-                      reinterpret_cast<uint4*>(drows), named);
+                      reinterpret_cast<uint4*>(drows), named, err);
     return;
   }
   const int64_t t = int64_t(blockIdx.x) - fill_blocks;

@@ -1082,11 +1082,14 @@ int bwd_by_experts(RouterBwdArgs& a, cudaStream_t s) {
   return launch_bwd<T, 16, 3>(a, s);
 }
 
-int router_shape(int64_t n, int experts, int topk, int64_t ld, int dtype, int score) {
-  if (n < 0 || experts < 1 || topk < 1 || (dtype != MXG_DTYPE_BF16 && dtype != MXG_DTYPE_F16 && dtype != MXG_DTYPE_F32) ||
-      (score != MXG_SCORE_SOFTMAX && score != MXG_SCORE_SIGMOID))
+int router_shape(const mxg_router_args* a) {
+  if (!a) return MXG_ERR_INVALID_ARGUMENT;
+  if (a->n_tokens < 0 || a->num_experts < 1 || a->topk < 1 ||
+      (a->dtype != MXG_DTYPE_BF16 && a->dtype != MXG_DTYPE_F16 && a->dtype != MXG_DTYPE_F32) ||
+      (a->score != MXG_SCORE_SOFTMAX && a->score != MXG_SCORE_SIGMOID) || !(a->scale > 0.0f) || !std::isfinite(a->scale))
     return MXG_ERR_INVALID_ARGUMENT;
-  if (experts > MXG_EP_MAX_EXPERTS || topk > experts || topk > MXG_ROUTER_MAX_TOPK || n > INT32_MAX || ld < experts)
+  if (a->num_experts > MXG_EP_MAX_EXPERTS || a->topk > a->num_experts || a->topk > MXG_ROUTER_MAX_TOPK ||
+      a->n_tokens > INT32_MAX || a->ld < a->num_experts)
     return MXG_ERR_BAD_SHAPE;
   return MXG_OK;
 }
@@ -1095,50 +1098,47 @@ int router_shape(int64_t n, int experts, int topk, int64_t ld, int dtype, int sc
 
 using namespace mxg;
 
-extern "C" int mxg_router_topk(const void* logits, int64_t ld, int dtype, int64_t n_tokens, int num_experts, int topk,
-                               int score, const float* bias, int groups, int topk_groups, int group_score,
-                               int renormalize, float scale, float* weights, int32_t* ids, void* stream) {
-  int st = router_shape(n_tokens, num_experts, topk, ld, dtype, score);
+extern "C" int mxg_router_topk(const mxg_router_args* args, void* stream) {
+  int st = router_shape(args);
   if (st) return st;
-  if (groups < 1 || topk_groups < 1 || topk_groups > groups ||
-      (group_score != MXG_GROUP_MAX && group_score != MXG_GROUP_TOP2) || !(scale > 0.0f) || !std::isfinite(scale))
+  const mxg_router_args& r = *args;
+  if (r.groups < 1 || r.topk_groups < 1 || r.topk_groups > r.groups ||
+      (r.group_score != MXG_GROUP_MAX && r.group_score != MXG_GROUP_TOP2))
     return MXG_ERR_INVALID_ARGUMENT;
-  if (groups > MXG_ROUTER_MAX_GROUPS || num_experts % groups || topk > topk_groups * (num_experts / groups))
+  if (r.groups > MXG_ROUTER_MAX_GROUPS || r.num_experts % r.groups ||
+      r.topk > r.topk_groups * (r.num_experts / r.groups))
     return MXG_ERR_BAD_SHAPE;
-  if (n_tokens == 0) return MXG_OK;
-  if (!logits || !weights || !ids) return MXG_ERR_INVALID_ARGUMENT;
+  if (r.n_tokens == 0) return MXG_OK;
+  if (!r.logits || !r.weights || !r.ids) return MXG_ERR_INVALID_ARGUMENT;
   if ((st = check_device())) return st;
   RouterArgs a{};
-  a.z = logits, a.ld = ld, a.n = n_tokens, a.experts = num_experts, a.topk = topk;
-  a.groups = topk_groups == groups ? 1 : groups;  // all groups stay: no groups
-  a.topk_groups = topk_groups == groups ? 1 : topk_groups;
-  a.top2 = group_score == MXG_GROUP_TOP2, a.sigmoid = score == MXG_SCORE_SIGMOID, a.renorm = renormalize != 0;
-  a.scale = scale, a.bias = bias, a.weights = weights, a.ids = ids;
-  a.rounds = topk + (bias && topk < a.topk_groups * (num_experts / a.groups) ? 1 : 0);
+  a.z = r.logits, a.ld = r.ld, a.n = r.n_tokens, a.experts = r.num_experts, a.topk = r.topk;
+  a.groups = r.topk_groups == r.groups ? 1 : r.groups;  // all groups stay: no groups
+  a.topk_groups = r.topk_groups == r.groups ? 1 : r.topk_groups;
+  a.top2 = r.group_score == MXG_GROUP_TOP2, a.sigmoid = r.score == MXG_SCORE_SIGMOID, a.renorm = r.renormalize != 0;
+  a.scale = r.scale, a.bias = r.bias, a.weights = r.weights, a.ids = r.ids;
+  a.rounds = r.topk + (r.bias && r.topk < a.topk_groups * (r.num_experts / a.groups) ? 1 : 0);
   cudaStream_t s = (cudaStream_t)stream;
-  return dtype == MXG_DTYPE_BF16  ? topk_by_experts<__nv_bfloat16>(a, s)
-         : dtype == MXG_DTYPE_F16 ? topk_by_experts<__half>(a, s)
-                                  : topk_by_experts<float>(a, s);
+  return r.dtype == MXG_DTYPE_BF16  ? topk_by_experts<__nv_bfloat16>(a, s)
+         : r.dtype == MXG_DTYPE_F16 ? topk_by_experts<__half>(a, s)
+                                    : topk_by_experts<float>(a, s);
 }
 
-extern "C" int mxg_router_topk_bwd(const void* logits, int64_t ld, int dtype, int64_t n_tokens, int num_experts,
-                                   int topk, int score, int renormalize, float scale, const float* weights,
-                                   const int32_t* ids, const float* dweights, void* dlogits, int64_t ld_out,
-                                   void* stream) {
-  int st = router_shape(n_tokens, num_experts, topk, ld, dtype, score);
+extern "C" int mxg_router_topk_bwd(const mxg_router_args* args, void* stream) {
+  int st = router_shape(args);
   if (st) return st;
-  if (!(scale > 0.0f) || !std::isfinite(scale)) return MXG_ERR_INVALID_ARGUMENT;
-  if (ld_out < num_experts) return MXG_ERR_BAD_SHAPE;
-  if (n_tokens == 0) return MXG_OK;
-  if (!logits || !weights || !ids || !dweights || !dlogits) return MXG_ERR_INVALID_ARGUMENT;
+  const mxg_router_args& r = *args;
+  if (r.ld_out < r.num_experts) return MXG_ERR_BAD_SHAPE;
+  if (r.n_tokens == 0) return MXG_OK;
+  if (!r.logits || !r.weights || !r.ids || !r.dweights || !r.dlogits) return MXG_ERR_INVALID_ARGUMENT;
   if ((st = check_device())) return st;
   RouterBwdArgs a{};
-  a.z = logits, a.ld = ld, a.n = n_tokens, a.ld_out = ld_out, a.experts = num_experts, a.topk = topk;
-  a.sigmoid = score == MXG_SCORE_SIGMOID, a.renorm = renormalize != 0, a.scale = scale;
-  a.weights = weights, a.ids = ids, a.dweights = dweights, a.dz = dlogits, a.err = device_error_word();
+  a.z = r.logits, a.ld = r.ld, a.n = r.n_tokens, a.ld_out = r.ld_out, a.experts = r.num_experts, a.topk = r.topk;
+  a.sigmoid = r.score == MXG_SCORE_SIGMOID, a.renorm = r.renormalize != 0, a.scale = r.scale;
+  a.weights = r.weights, a.ids = r.ids, a.dweights = r.dweights, a.dz = r.dlogits, a.err = device_error_word();
   if (!a.err) return MXG_ERR_CUDA;
   cudaStream_t s = (cudaStream_t)stream;
-  return dtype == MXG_DTYPE_BF16  ? bwd_by_experts<__nv_bfloat16>(a, s)
-         : dtype == MXG_DTYPE_F16 ? bwd_by_experts<__half>(a, s)
-                                  : bwd_by_experts<float>(a, s);
+  return r.dtype == MXG_DTYPE_BF16  ? bwd_by_experts<__nv_bfloat16>(a, s)
+         : r.dtype == MXG_DTYPE_F16 ? bwd_by_experts<__half>(a, s)
+                                    : bwd_by_experts<float>(a, s);
 }

@@ -289,17 +289,18 @@ def swiglu_bwd(gu: torch.Tensor, dh: torch.Tensor) -> torch.Tensor:
 
 
 # ---------------------------------------------------------------- router
-def _logits(logits, name="logits"):
-    """(tensor whose rows are contiguous, row stride)"""
+def _logits(logits):
+    """(tensor whose rows are contiguous, row stride, tokens, experts)"""
     if logits.dtype not in _LOGITS or logits.dim() != 2:
-        raise TypeError(f"{name} must be a 2-D bf16, fp16 or fp32 tensor")
+        raise TypeError("logits must be a 2-D bf16, fp16 or fp32 tensor")
     n, E = logits.shape
     if not 1 <= E <= _lib.EP_MAX_EXPERTS:
-        raise ValueError(f"{name} has {E} experts, 1 to {_lib.EP_MAX_EXPERTS} are supported")
-    _cuda(logits, name)
-    if logits.stride(1) != 1 or logits.stride(0) < E:
-        logits = logits.contiguous()
-    return logits, logits.stride(0)
+        raise ValueError(f"logits has {E} experts, 1 to {_lib.EP_MAX_EXPERTS} are supported")
+    _cuda(logits, "logits")
+    ld, one = logits.stride()
+    if one != 1 or ld < E:
+        logits, ld = logits.contiguous(), E
+    return logits, ld, n, E
 
 
 def _per_choice(t, name, dtype, like):
@@ -337,16 +338,16 @@ def router_topk(logits: torch.Tensor, topk: int, *, score: str = "softmax", bias
     ``combine`` the weights.  The differentiable form is
     ``autograd.router_topk``."""
     code = _score(score, scale)
-    if group_score not in _GROUP_SCORES:
+    by = _GROUP_SCORES.get(group_score)
+    if by is None:
         raise ValueError(f"group_score must be 'max' or 'top2', got {group_score!r}")
     if topk_groups is None:
         topk_groups = groups
-    logits, ld = _logits(logits)
-    n, E = logits.shape
+    logits, ld, n, E = _logits(logits)
     if not 1 <= groups <= _lib.ROUTER_MAX_GROUPS or E % groups or not 1 <= topk_groups <= groups:
         raise ValueError(f"groups={groups} (at most {_lib.ROUTER_MAX_GROUPS}) must divide {E} experts and "
                          f"topk_groups={topk_groups} lie in 1..groups")
-    if not 1 <= topk <= min(_lib.ROUTER_MAX_TOPK, topk_groups * (E // groups)):
+    if not (1 <= topk <= _lib.ROUTER_MAX_TOPK and topk <= topk_groups * (E // groups)):
         raise ValueError(f"topk={topk} must lie in 1..{min(_lib.ROUTER_MAX_TOPK, topk_groups * (E // groups))}")
     dev = logits.device
     if bias is not None:
@@ -355,9 +356,9 @@ def router_topk(logits: torch.Tensor, topk: int, *, score: str = "softmax", bias
             raise ValueError("bias and logits must be on one device")
     weights = torch.empty(n, topk, dtype=torch.float32, device=dev)
     ids = torch.empty(n, topk, dtype=torch.int32, device=dev)
-    _lib.launch("mxg_router_topk", dev, logits.data_ptr(), ld, _LOGITS[logits.dtype], n, E, topk, code,
-                _lib.ptr(bias), groups, topk_groups, _GROUP_SCORES[group_score], renormalize, scale,
-                weights.data_ptr(), ids.data_ptr())
+    _lib.launch("mxg_router_topk", dev, _lib.router_args(
+        logits.data_ptr(), 0 if bias is None else bias.data_ptr(), weights.data_ptr(), ids.data_ptr(), 0, 0, n, ld, E,
+        _LOGITS[logits.dtype], E, topk, code, groups, topk_groups, by, renormalize, scale, 0))
     return weights, ids
 
 
@@ -369,8 +370,7 @@ def router_topk_bwd(logits: torch.Tensor, weights: torch.Tensor, ids: torch.Tens
     bias or the grouping).  An id out of range is skipped and sets the device
     error word; an id named twice in a row gets the sum."""
     code = _score(score, scale)
-    logits, ld = _logits(logits)
-    n, E = logits.shape
+    logits, ld, n, E = _logits(logits)
     if weights.dim() != 2 or weights.shape[0] != n or not 1 <= weights.shape[1] <= min(E, _lib.ROUTER_MAX_TOPK):
         raise ValueError(f"weights has shape {tuple(weights.shape)}, expected ({n}, topk)")
     if ids.dtype != torch.int32:
@@ -382,8 +382,9 @@ def router_topk_bwd(logits: torch.Tensor, weights: torch.Tensor, ids: torch.Tens
     if not weights.device == ids.device == dweights.device == dev:
         raise ValueError("logits, weights, ids and dweights must be on one device")
     out = torch.empty(n, E, dtype=logits.dtype, device=dev)
-    _lib.launch("mxg_router_topk_bwd", dev, logits.data_ptr(), ld, _LOGITS[logits.dtype], n, E, shape[1], code,
-                renormalize, scale, weights.data_ptr(), ids.data_ptr(), dweights.data_ptr(), out.data_ptr(), E)
+    _lib.launch("mxg_router_topk_bwd", dev, _lib.router_args(
+        logits.data_ptr(), 0, weights.data_ptr(), ids.data_ptr(), dweights.data_ptr(), out.data_ptr(), n, ld, E,
+        _LOGITS[logits.dtype], E, shape[1], code, 1, 1, 0, renormalize, scale, 0))
     return out
 
 
@@ -426,7 +427,8 @@ def combine_bwd(dout: torch.Tensor, rows: torch.Tensor, slot_pos: torch.Tensor, 
 
     A negative position has no row (its dweights are 0); one beyond the rows
     is skipped too and sets the device error word.  slot_pos names a row at
-    most once; a row that it does not name has gradient 0."""
+    most once, as ``CudaEpOps.route`` gives it (one named twice sets the error
+    word); a row that it does not name has gradient 0."""
     rows, slot_pos, weights = _combine_args(rows, slot_pos, weights)
     (n, k), (P, H), dev = slot_pos.shape, rows.shape, rows.device
     if dout.dtype != torch.bfloat16 or dout.shape != (n, H) or dout.device != dev:

@@ -46,7 +46,8 @@ class AdamW:
     multiple of 256, and zeros fill the gaps.  The step count lives on the
     device, so a captured ``step`` counts on at every replay; ``lr`` may be a
     number (fixed at capture) or a one-element fp32 CUDA tensor that is read
-    at every step.  One optimiser's steps run one after the other: do not
+    at every step.  ``lr``, ``betas``, ``eps`` and ``weight_decay`` may be set
+    between steps.  One optimiser's steps run one after the other: do not
     issue them on several streams at once."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay=0.01, *,
@@ -60,11 +61,7 @@ class AdamW:
             raise ValueError(f"betas must lie in [0, 1), got {betas}")
         if not eps > 0.0:
             raise ValueError(f"eps must be positive, got {eps}")
-        decay = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * len(params)
-        if len(decay) != len(params):
-            raise ValueError(f"{len(decay)} weight decays for {len(params)} tensors")
-        if not all(d >= 0.0 for d in decay):
-            raise ValueError("weight_decay must not be negative")
+        decay = self._decays(weight_decay, len(params))
         for i, p in enumerate(params):
             if p.dtype not in _GRAD:
                 raise TypeError(f"params[{i}] must be bf16 or fp32, got {p.dtype}")
@@ -116,8 +113,18 @@ class AdamW:
         self._chunks = torch.from_numpy(table if table.size else np.zeros(1, np.int32)).to(dev)
         self._lay_out()
 
+    @staticmethod
+    def _decays(weight_decay, count):
+        decay = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * count
+        if len(decay) != count:
+            raise ValueError(f"{len(decay)} weight decays for {count} tensors")
+        if not all(d >= 0.0 for d in decay):
+            raise ValueError("weight_decay must not be negative")
+        return decay
+
     def _lay_out(self):
-        """The device table of the tensors (again when one has moved)."""
+        """The device table of the tensors (again when one has moved, or a weight decay changed)."""
+        self.weight_decay = self._decays(self.weight_decay, len(self.params))
         for i, (p, shape) in enumerate(zip(self.params, self._shapes)):
             if p.shape != shape or p.dtype != self._dtypes[i] or p.device != self.device or not p.is_contiguous():
                 raise ValueError(f"params[{i}] is no longer a contiguous {tuple(shape)} {self._dtypes[i]} tensor on "
@@ -141,7 +148,7 @@ class AdamW:
             grads = [p.grad for p in params]
         elif len(grads) != len(params):
             raise ValueError(f"{len(grads)} gradients for {len(params)} tensors")
-        lr, lr_ptr = self.lr, None
+        lr, lr_ptr = self.lr, 0
         if isinstance(lr, torch.Tensor):
             if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != self.device:
                 raise ValueError(f"lr must be a number or a one-element fp32 tensor on {self.device}")
@@ -160,13 +167,15 @@ class AdamW:
                         np.uint64)
         if list(map(_data_ptr, params)) != self._at or self.weight_decay != self._laid_out:
             if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("a tensor moved since the last step: take one step before the capture")
+                raise RuntimeError("a tensor moved, or a weight decay changed, since the last step: take one step "
+                                   "before the capture")
             self._lay_out()
-        _lib.launch("mxg_adamw_step", self.device, self._table.data_ptr(), len(params), self._chunks.data_ptr(),
-                    self._chunk_begin.ctypes.data, self._chunk, ptrs.ctypes.data, kinds.ctypes.data, self.state_bits,
-                    self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), _lib.ptr(self.exp_avg_scale),
-                    _lib.ptr(self.exp_avg_sq_scale), _lib.ptr(self.master), self._step.data_ptr(),
-                    self._done.data_ptr(), lr, lr_ptr, self.betas[0], self.betas[1], self.eps, self.seed)
+        at = lambda t: 0 if t is None else t.data_ptr()
+        _lib.launch("mxg_adamw_step", self.device, _lib.adamw_args(
+            at(self._table), at(self._chunks), self._chunk_begin.ctypes.data, ptrs.ctypes.data, kinds.ctypes.data,
+            at(self.exp_avg), at(self.exp_avg_sq), at(self.exp_avg_scale), at(self.exp_avg_sq_scale), at(self.master),
+            at(self._step), at(self._done), lr_ptr, lr, *self.betas, self.eps, self.seed, len(params), self._chunk,
+            self.state_bits, 0))
         del held
         tracked = [p for p in params if p.requires_grad]
         if tracked:                                # autograd sees the change in place

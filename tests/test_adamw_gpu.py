@@ -236,6 +236,41 @@ def test_moved_weights_and_grad_attribute(mxg, cuda_dev):
             opt.step(bad)
 
 
+def test_settings_changed_between_steps(mxg, cuda_dev):
+    p = _make([(300,), (4097,)], [F32, BF], 24, cuda_dev)
+    mirror = Mirror(mxg.optim.AdamW(p))
+    opt = mirror.opt
+    for t, (lr, decay, betas) in enumerate([(1e-3, 0.1, (0.9, 0.999)), (0.0, [0.0, 0.5], (0.9, 0.999)),
+                                            (3e-2, 0.0, (0.0, 0.5)), (1e-4, 0.2, (0.5, 0.0))]):
+        opt.lr, opt.weight_decay, opt.betas = lr, decay, betas
+        if not isinstance(decay, list):
+            opt.weight_decay = [decay, decay] if t % 2 else decay
+        k = opt.weight_decay
+        opt.weight_decay = k
+        grads = _make([(300,), (4097,)], [F32, BF], 30 + t, cuda_dev, std=1e-2)
+        if not isinstance(k, list):
+            opt._lay_out()                        # what the step does: one number for every tensor
+        mirror.step(grads)
+    opt.weight_decay = [0.1]
+    with pytest.raises(ValueError, match="decay"):
+        opt.step(grads)
+    opt.weight_decay, opt.eps = 0.1, 0.0
+    with pytest.raises(mxg.MxgError):
+        opt.step(grads)
+
+
+def test_nothing_to_do(mxg, cuda_dev):
+    p = [torch.empty(0, device=cuda_dev), torch.empty(0, 7, device=cuda_dev)]
+    opt = mxg.optim.AdamW(p)
+    opt.step([torch.empty(0, device=cuda_dev), None])
+    assert opt.state_dict()["step"] == 1
+    q = _make([(40,)], [BF], 25, cuda_dev)
+    keep = q[0].clone()
+    opt = mxg.optim.AdamW(q, state_bits=8)
+    opt.step([None])
+    assert torch.equal(q[0], keep) and opt.state_dict()["step"] == 1
+
+
 def test_another_stream(mxg, cuda_dev):
     a, b = _make([(5000,)], [BF], 15, cuda_dev), _make([(5000,)], [BF], 15, cuda_dev)
     g = _make([(5000,)], [BF], 16, cuda_dev)

@@ -1,5 +1,8 @@
 """Argument checks of the router, the combine's gradient and AdamW, and the
 8-bit codes, on a machine without a GPU."""
+import os
+import subprocess
+
 import numpy as np
 import pytest
 import torch
@@ -31,20 +34,23 @@ def test_router_refuses_bad_arguments(mxg):
 
 
 def test_router_abi_refuses_bad_shapes(mxg):
-    L = mxg._lib.load()
+    L, pack = mxg._lib.load(), mxg._lib.router_args
 
     def call(ld=64, dtype=1, n=4, E=64, k=4, score=0, groups=1, kept=1, gs=0, scale=1.0, z=16):
-        return L.mxg_router_topk(z, ld, dtype, n, E, k, score, None, groups, kept, gs, 1, scale, 16, 16, None)
+        return L.mxg_router_topk(pack(z, 0, 16, 16, 0, 0, n, ld, E, dtype, E, k, score, groups, kept, gs, 1, scale, 0),
+                                 None)
     assert call(n=0) == 0
     assert call(n=-1) == 1 and call(E=0) == 1 and call(k=0) == 1 and call(dtype=3) == 1 and call(score=2) == 1
     assert call(E=385, ld=385) == 2 and call(k=65) == 2 and call(k=33) == 2 and call(ld=63) == 2
     assert call(groups=0) == 1 and call(groups=4, kept=5) == 1 and call(gs=2) == 1 and call(scale=-1.0) == 1
-    assert call(scale=float("nan")) == 1 and call(z=None) == 1
+    assert call(scale=float("nan")) == 1 and call(z=0) == 1
     assert call(groups=5) == 2 and call(groups=64, kept=64) == 2
     assert call(groups=16, kept=1, k=5) == 2                   # four experts are left
+    assert L.mxg_router_topk(None, None) == 1 and L.mxg_router_topk_bwd(None, None) == 1
+
     def bwd(ld=64, n=4, E=64, k=4, ld_out=64, scale=1.0, w=16):
-        return L.mxg_router_topk_bwd(16, ld, 1, n, E, k, 0, 1, scale, w, 16, 16, 16, ld_out, None)
-    assert bwd(n=0) == 0 and bwd(ld_out=60) == 2 and bwd(scale=0.0) == 1 and bwd(w=None) == 1 and bwd(k=65) == 2
+        return L.mxg_router_topk_bwd(pack(16, 0, w, 16, 16, 16, n, ld, ld_out, 1, E, k, 0, 0, 0, 0, 1, scale, 0), None)
+    assert bwd(n=0) == 0 and bwd(ld_out=60) == 2 and bwd(scale=0.0) == 1 and bwd(w=0) == 1 and bwd(k=65) == 2
 
 
 def test_combine_gradient_refuses_bad_arguments(mxg):
@@ -92,11 +98,13 @@ def test_adamw_abi_refuses_bad_arguments(mxg):
     L = mxg._lib.load()
     begin, grads, kinds = np.zeros(2, np.int64), np.array([16], np.uint64), np.array([1], np.int32)
 
-    def call(n=1, bits=32, m=16, ms=None, lr=1e-3, b1=0.9, b2=0.99, eps=1e-8, grads=grads, kinds=kinds, begin=begin,
+    def call(n=1, bits=32, m=16, ms=0, lr=1e-3, b1=0.9, b2=0.99, eps=1e-8, grads=grads, kinds=kinds, begin=begin,
              step=16, chunk=4096):
-        return L.mxg_adamw_step(16, n, 16, begin.ctypes.data, chunk, grads.ctypes.data, kinds.ctypes.data, bits, m, 16, ms,
-                                ms, None, step, 16, lr, None, b1, b2, eps, 0, None)
-    assert call(n=0) == 1 and call(bits=16) == 1 and call(m=None) == 1 and call(step=None) == 1
+        return L.mxg_adamw_step(mxg._lib.adamw_args(
+            16, 16, begin.ctypes.data, grads.ctypes.data, kinds.ctypes.data, m, 16, ms, ms, 0, step, 16, 0, lr, b1, b2,
+            eps, 0, n, chunk, bits, 0), None)
+    assert L.mxg_adamw_step(None, None) == 1
+    assert call(n=0) == 1 and call(bits=16) == 1 and call(m=0) == 1 and call(step=0) == 1
     assert call(bits=8) == 1                                     # no scales
     assert call(chunk=0) == 1 and call(chunk=4000) == 1
     assert call(lr=-1.0) == 1 and call(b1=1.0) == 1 and call(b2=-0.1) == 1 and call(eps=float("nan")) == 1
@@ -108,12 +116,23 @@ def test_adamw_abi_refuses_bad_arguments(mxg):
     assert L.mxg_adamw_moments(16, None, 16, 16, 256, 16, 16, None) == 1
 
 
-def test_tensor_table_matches_the_header(mxg):
-    """The field offsets of mxg_adamw_tensor as a C compiler lays them out."""
+def test_argument_layouts_match_the_header(mxg, tmp_path):
+    """Sizes and field offsets as the C compiler lays the structs out."""
+    assert len(mxg._lib.router_args(*[0] * 17, 1.0, 0)) == 6 * 8 + 3 * 8 + 8 * 4 + 8
+    assert len(mxg._lib.adamw_args(*[0] * 13, *[0.0] * 4, *[0] * 5)) == 13 * 8 + 4 * 8 + 8 + 4 * 4
     e = mxg.optim._ENTRY
     assert e.itemsize == 48
     assert [e.fields[n][1] for n in ("param", "numel", "offset", "master", "decay", "kind", "first_chunk")] == \
         [0, 8, 16, 24, 32, 36, 40]
+    source = tmp_path / "sizes.c"
+    source.write_text('#include <stdio.h>\n#include "mxg.h"\nint main(void) { printf("%zu %zu %zu %zu %zu %zu", '
+                      'sizeof(mxg_router_args), offsetof(mxg_router_args, scale), sizeof(mxg_adamw_args), '
+                      'offsetof(mxg_adamw_args, seed), sizeof(mxg_adamw_tensor), '
+                      'offsetof(mxg_adamw_tensor, first_chunk)); return 0; }')
+    subprocess.run(["gcc", "-I", os.path.dirname(mxg._lib.HEADER_PATH), str(source), "-o", str(tmp_path / "sizes")],
+                   check=True)
+    sizes = subprocess.run([str(tmp_path / "sizes")], check=True, capture_output=True, text=True).stdout
+    assert sizes.split() == ["112", "104", "160", "136", "48", "40"]
     text = open(mxg._lib.HEADER_PATH).read()
     for name, value in (("MXG_ADAMW_BLOCK", 256), ("MXG_ROUTER_MAX_TOPK", 32),
                         ("MXG_ROUTER_MAX_GROUPS", 32), ("MXG_EP_MAX_EXPERTS", 384)):

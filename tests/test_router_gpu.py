@@ -346,6 +346,16 @@ def test_combine_gradient_skips_positions_beyond_the_rows(mxg, cuda_dev):
     assert mxg.device_error() == mxg._lib.MXG_ERR_INVALID_ARGUMENT
 
 
+def test_combine_gradient_reports_a_row_named_twice(mxg, cuda_dev):
+    dout, rows, pos, w = _combine_inputs(40, 2, 64, 80, 2, cuda_dev)
+    pos[7, 0] = pos[30, 1]
+    drows, dw = mxg.ops.combine_bwd(dout, rows, pos, w)
+    assert mxg.device_error() == mxg._lib.MXG_ERR_INVALID_ARGUMENT
+    at = int(pos[7, 0])
+    either = [(w[t, j] * dout[t].float()).to(torch.bfloat16) for t, j in ((7, 0), (30, 1))]
+    assert torch.all((drows[at] == either[0]) | (drows[at] == either[1])) and torch.isfinite(dw).all()
+
+
 def test_combine_gradient_without_tokens(mxg, cuda_dev):
     rows = torch.ones(3, 16, dtype=torch.bfloat16, device=cuda_dev)
     drows, dw = mxg.ops.combine_bwd(rows[:0], rows, torch.empty(0, 2, dtype=torch.int32, device=cuda_dev))
