@@ -85,7 +85,10 @@ def router_topk(logits: torch.Tensor, topk: int, *, score: str = "softmax", bias
                 scale: float = 1.0):
     """``ops.router_topk`` with a gradient: (weights [n, topk] fp32, ids [n, topk]
     int32) of logits [n, E]; the weights' gradient flows to the logits, the
-    choice (ids, bias, groups) has none."""
+    choice (ids, bias, groups) has none.  As with any torch operation, capture
+    a backward pass with ``torch.autograd.grad`` while no eager graph of the
+    same leaves is alive; ``ops.router_topk_bwd`` and ``ops.combine_bwd`` can be
+    captured freely."""
     return _RouterTopk.apply(logits, topk, score, bias, groups, topk_groups, group_score, renormalize, scale)
 
 

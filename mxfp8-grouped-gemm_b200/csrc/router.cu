@@ -278,9 +278,9 @@ __device__ __noinline__ bool order_near(const RouterArgs& a, const T* row, float
     if (in && at < 32) list[at] = uint32_t(e);
     count += __popc(all);
   }
+  __syncwarp();
   if (count > 32 || count < a.topk) return false;
   if (a.bias && !a.sigmoid) sum = lanes_sum<32>(sum);
-  __syncwarp();
   const int e = lane < count ? int(list[lane]) : 0;  // ascending: the lower lane has the lower index
   double x = double(to_f32(row[e]));
   if (a.bias) x = (a.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - double(base)) / sum) + double(a.bias[e]);

@@ -393,3 +393,31 @@ def test_router_and_combine_through_autograd(mxg, cuda_dev):
     size = np.abs(ref_dw).max(1, keepdims=True)
     assert np.all(np.abs(_np(z.grad) - ref_z) <= 4 * G_TOL * size)
     assert mxg.device_error() == 0
+
+
+def test_captured_backward_pass(mxg, cuda_dev):
+    """Forward and backward through autograd in one graph, replayed on new inputs."""
+    n, E, k, H = 40, 64, 4, 64
+    z = _logits(n, E, "fp32", 3, cuda_dev).requires_grad_(True)
+    rows = torch.randn(n * k, H, device=cuda_dev).to(torch.bfloat16).requires_grad_(True)
+    pos = torch.randperm(n * k, device=cuda_dev).to(torch.int32).view(n, k)
+    up = torch.randn(n, H, device=cuda_dev).to(torch.bfloat16)
+
+    def both():
+        w, _ = mxg.router_topk(z, k, score="sigmoid")
+        return torch.autograd.grad(mxg.combine(rows, pos, w), (z, rows), up)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = both()
+    with torch.no_grad():
+        z.copy_(_logits(n, E, "fp32", 4, cuda_dev))
+        rows.mul_(2)
+    graph.replay()
+    want = both()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert mxg.device_error() == 0
