@@ -471,6 +471,8 @@ __global__ void __launch_bounds__(kRouterThreads) router_topk_kernel(const __gri
       head = code < V * 256 ? next[code >> 8] : -INFINITY;
     }
   }
+  // the best of what no round named: the order of the last choices is certain against it too
+  const float after = a.bias ? lanes_max<LANES>(head) : -INFINITY;
   __syncwarp();
   auto expert = [&](float2 c) {  // index of a choice
     const int l = __float_as_int(c.y) & 255;
@@ -496,10 +498,13 @@ __global__ void __launch_bounds__(kRouterThreads) router_topk_kernel(const __gri
     s_id[sub][q] = e;
     if (a.bias && q + 1 < rounds) {
       const float2 d = rec[q + 1];
-      if (!(c.x - d.x > near + 0x1p-23f * (fabsf(c.x) + fabsf(d.x)))) {
-        // the same logit and the same bias tie for certain, and stand in order of index
+      auto apart = [&](float u, float v) { return u - v > near + 0x1p-23f * (fabsf(u) + fabsf(v)); };
+      if (!apart(c.x, d.x)) {
+        // the same logit and the same bias tie for certain, and stand in order
+        // of index; the last choice only where what follows the two is apart
         const int j = expert(d);
         if (!(to_f32(row[e]) == to_f32(row[j]) && a.bias[e] == a.bias[j])) again = true;
+        if (q == k - 1 && !apart(d.x, after)) again = true;
       }
     }
   }
@@ -741,9 +746,10 @@ __global__ void __launch_bounds__(kRouterThreads) router_rows_kernel(const __gri
     if (!exact && q < k) {
       again |= mine < kNoStep;
       if (then != 0 && float((mine >> IB) - (then >> IB)) <= near * steps + (a.bias ? 1.0f : 0.0f)) {
-        // the same logit and the same bias tie for certain, and stand in order of index
+        // the same logit and the same bias tie for certain, and stand in order
+        // of index; not so for the last choice, where a later one may pass both
         const int e = id[i], f = int(kLast - (then & kLast));
-        if (!(to_f32(row[e]) == to_f32(row[f]) && (!a.bias || a.bias[e] == a.bias[f]))) close = true;
+        if (q == k - 1 || !(to_f32(row[e]) == to_f32(row[f]) && (!a.bias || a.bias[e] == a.bias[f]))) close = true;
       }
     }
     s_id[warp][sub][q] = id[i];

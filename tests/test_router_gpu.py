@@ -130,6 +130,28 @@ def test_choices_that_32_bits_cannot_tell_apart(mxg, cuda_dev):
                group_score="top2")
 
 
+@pytest.mark.parametrize("E", [64, 256, 384])
+@pytest.mark.parametrize("n", [40, 8200])
+def test_equal_experts_at_the_last_choice(mxg, cuda_dev, E, n):
+    """Two equal experts stand on either side of the last choice, and a later
+    one is larger by the last place of fp32: it comes before both."""
+    g = torch.Generator(device=cuda_dev).manual_seed(E + n)
+    z = torch.rand(n, E, generator=g, device=cuda_dev)
+    for k, equal in ((1, 2), (3, 2), (3, 4), (8, 2), (8, 3), (8, 12)):
+        # `equal` experts at 1.5, the last of them one place higher, and k - 1 above
+        at = torch.rand(n, E, generator=g, device=cuda_dev).argsort(1)
+        ties = at[:, :equal + 1].sort(1).values
+        near = z.scatter(1, ties, 1.5)
+        near.scatter_(1, ties[:, -1:], 1.5 + 2.0 ** -23)
+        near.scatter_(1, at[:, equal + 1:equal + k], 2.0 + z[:, :k - 1])
+        bias = torch.full((E,), 0.25, device=cuda_dev)
+        _check(mxg, near, k)
+        for score in ("softmax", "sigmoid"):
+            _check(mxg, near, k, score=score, bias=bias)
+        if E == 256:
+            _check(mxg, near, k, score="sigmoid", bias=bias, groups=8, topk_groups=8)
+
+
 @pytest.mark.parametrize("E", [8, 64, 160, 256])
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_masked_experts_and_rows(mxg, cuda_dev, E, score):
