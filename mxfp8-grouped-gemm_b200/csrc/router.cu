@@ -283,7 +283,11 @@ __device__ __noinline__ bool order_near(const RouterArgs& a, const T* row, float
   if (a.bias && !a.sigmoid) sum = lanes_sum<32>(sum);
   const int e = lane < count ? int(list[lane]) : 0;  // ascending: the lower lane has the lower index
   double x = double(to_f32(row[e]));
-  if (a.bias) x = (a.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - double(base)) / sum) + double(a.bias[e]);
+  if (a.bias) {
+    if (a.sigmoid) x = 1.0 / (1.0 + exp(-x));
+    else x = sum > 0.0 ? exp(x - double(base)) / sum : 0.0;          // a row without an expert has no score
+    x += double(a.bias[e]);
+  }
   int rank = 0;
   for (int i = 0; i < count; ++i) {
     const double o = __shfl_sync(kFull, x, i);
@@ -640,7 +644,7 @@ __global__ void __launch_bounds__(kRouterThreads) router_rows_kernel(const __gri
   // values of 16 below the largest logit, of 2 below the largest s + bias,
   // share the lowest step: where that is chosen, the slow selection decides
   const float scale = a.bias ? 0.5f : 0.0625f, steps = scale * float(1u << (31 - IB));
-  const float shift = (1.0f - 0x1p-22f) - largest * scale;
+  const float shift = __fmaf_rd(-largest, scale, 1.0f - 0x1p-22f);  // down: no value reaches 1
   uint32_t key[NC][8];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {

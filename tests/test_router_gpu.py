@@ -152,6 +152,22 @@ def test_equal_experts_at_the_last_choice(mxg, cuda_dev, E, n):
             _check(mxg, near, k, score="sigmoid", bias=bias, groups=8, topk_groups=8)
 
 
+@pytest.mark.parametrize("E", [16, 40, 256, 384])
+@pytest.mark.parametrize("n", [20, 8200])
+def test_logits_and_biases_far_from_zero(mxg, cuda_dev, E, n):
+    """Softmax does not change with an offset, the choice does not with either."""
+    g = torch.Generator(device=cuda_dev).manual_seed(E)
+    z = torch.randn(n, E, generator=g, device=cuda_dev).mul_(1.5)
+    b = torch.randn(E, generator=g, device=cuda_dev)
+    for off in (-1e4, -300.0, -61.7, 61.7, 5e3, 1e30):
+        _check(mxg, z + off, 4)
+        _check(mxg, z + off, 8, renormalize=False)
+    for score in ("softmax", "sigmoid"):
+        for by in (3.0, 12.0, 1e3, 1e6):
+            _check(mxg, z, 4, score=score, bias=b * by)
+            _check(mxg, z, 8, score=score, bias=b + by)
+
+
 @pytest.mark.parametrize("E", [8, 64, 160, 256])
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_masked_experts_and_rows(mxg, cuda_dev, E, score):
@@ -184,6 +200,19 @@ def test_masked_experts_and_rows(mxg, cuda_dev, E, score):
     bias[1:5] = -inf                             # switched off by the bias
     _, ids = mxg.ops.router_topk(_logits(64, E, "bf16", 1, cuda_dev), 3, score=score, bias=bias)
     assert not torch.isin(ids, torch.arange(1, 5, device=cuda_dev)).any()
+
+
+@pytest.mark.parametrize("E", [17, 64, 256, 384])
+@pytest.mark.parametrize("n", [3, 8200])
+def test_rows_without_an_expert_go_by_the_bias(mxg, cuda_dev, E, n):
+    """Every score is 0: the order is the bias's, however close its values are."""
+    g = torch.Generator(device=cuda_dev).manual_seed(E)
+    z = torch.randn(n, E, generator=g, device=cuda_dev)
+    z[1::2] = -float("inf")
+    bias = torch.randint(-2, 3, (E,), generator=g, device=cuda_dev).float() * 1e-7
+    for score in ("softmax", "sigmoid"):
+        for k in (1, 4, 8):
+            _check(mxg, z, k, score=score, bias=bias)
 
 
 def test_nan_rows_have_ids_in_range(mxg, cuda_dev):
