@@ -534,7 +534,12 @@ __global__ void __launch_bounds__(kRouterThreads) router_topk_kernel(const __gri
 // steps of the value below the row's largest, over the index from the top
 // (16-bit logits without a bias: the 16 bits themselves, exact).  Every chunk
 // is sorted in a lane, then the eight largest are merged over the chunks and
-// over the lanes; what a merge leaves out is kept as one largest value.
+// over the lanes.  Of what the merges leave out the largest is kept, and with a
+// bias the two largest: where the first places of these ten that hold all the
+// choices are apart from the rest, a token whose order is in doubt is settled
+// by its own lanes among them, which costs the throughput 5% and saves a warp
+// that is alone on its token at the end: 16384 rows of 256, sigmoid, bias,
+// groups 18.6 -> 15.9 us; bf16 with a bias of zero (ties) 19.8 -> 16.6 at 8192.
 constexpr int kRowLanes = 4, kRowMost = 8;
 
 template <int A, int B>
@@ -551,13 +556,16 @@ __device__ __forceinline__ void sort_keys(uint32_t (&x)[8], std::index_sequence<
 __device__ __forceinline__ void sort_keys(uint32_t (&x)[8]) {
   sort_keys(x, std::make_index_sequence<Network<8>().n>());
 }
-// The 8 largest of two descending lists, descending; the largest of the others joins `out`.
-__device__ __forceinline__ void merge_keys(uint32_t (&x)[8], const uint32_t (&y)[8], uint32_t& out) {
+// The 8 largest of two descending lists, descending; the two largest of the
+// others join `out`, `out2` (with a bias: nothing else asks for them).
+template <bool BIAS>
+__device__ __forceinline__ void merge_keys(uint32_t (&x)[8], const uint32_t (&y)[8], uint32_t& out, uint32_t& out2) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const uint32_t a = x[i], b = y[7 - i];
+    const uint32_t a = x[i], b = y[7 - i], low = min(a, b);
     x[i] = max(a, b);
-    out = max(out, min(a, b));
+    if (BIAS) out2 = max(out2, min(out, low));
+    out = max(out, low);
   }
   order_keys<0, 4>(x), order_keys<1, 5>(x), order_keys<2, 6>(x), order_keys<3, 7>(x);
   order_keys<0, 2>(x), order_keys<1, 3>(x), order_keys<4, 6>(x), order_keys<5, 7>(x);
@@ -572,7 +580,13 @@ __device__ __forceinline__ uint32_t order16(float z) {
   return u & 0x8000u ? 0xFFFFu - u : u | 0x8000u;
 }
 
-template <typename T, int NC>
+// A choice's score + bias in fp64.
+template <typename T>
+__device__ __noinline__ double sigmoid_f64(const T* row, const float* bias, int e) {
+  return 1.0 / (1.0 + exp(-double(to_f32(row[e])))) + double(bias[e]);
+}
+
+template <typename T, int NC, bool BIAS>
 __global__ void __launch_bounds__(kRouterThreads) router_rows_kernel(const __grid_constant__ RouterArgs a) {
   constexpr int PER_WARP = 32 / kRowLanes, WARPS = kRouterThreads / 32;
   constexpr int IB = NC <= 8 ? 8 : 9;                    // bits of the index
@@ -580,13 +594,13 @@ __global__ void __launch_bounds__(kRouterThreads) router_rows_kernel(const __gri
   constexpr uint32_t kNoStep = 0x80000000u + (1u << IB);  // smaller keys: the lowest step
   __shared__ __align__(16) uint32_t s_list[WARPS][PER_WARP][12];
   __shared__ int32_t s_id[WARPS][PER_WARP][kRowMost];
-  __shared__ uint64_t s_key[WARPS][NC * 32];
+  __shared__ uint64_t s_key[WARPS][NC * 32 < 96 ? 96 : NC * 32];
   const int wl = threadIdx.x & 31, warp = threadIdx.x >> 5, lane = wl & (kRowLanes - 1), sub = wl / kRowLanes;
   const int64_t want = (int64_t(blockIdx.x) * WARPS + warp) * PER_WARP + sub;
   const int64_t r = want < a.n ? want : a.n - 1;
   const T* row = static_cast<const T*>(a.z) + r * a.ld;
   const int E = a.experts, k = a.topk, chunks = (E + 31) / 32;
-  const bool exact = sizeof(T) == 2 && !a.bias;
+  const bool exact = sizeof(T) == 2 && !BIAS;
 
   float x[NC][8];
   float top = -INFINITY;  // a NaN if there is one
@@ -604,7 +618,7 @@ __global__ void __launch_bounds__(kRouterThreads) router_rows_kernel(const __gri
   const float base = top == -INFINITY ? 0.0f : top;
   const bool odd = !a.sigmoid && !(top < INFINITY);  // a NaN or +inf: softmax has no value
   float inv = 0.0f;
-  if (!a.sigmoid && (a.bias || !a.renorm)) {
+  if (!a.sigmoid && (BIAS || !a.renorm)) {
     float sum = 0.0f;
 #pragma unroll
     for (int c = 0; c < NC; ++c)
@@ -612,15 +626,14 @@ __global__ void __launch_bounds__(kRouterThreads) router_rows_kernel(const __gri
       for (int v = 0; v < 8; ++v) {
         const float f = exp_fast(x[c][v] - base);
         sum += f;
-        if (a.bias) x[c][v] = f;
+        if (BIAS) x[c][v] = f;
       }
     sum = lanes_sum<kRowLanes>(sum);
     inv = sum > 0.0f ? 1.0f / sum : 0.0f;
   }
   float near = 0.0f, largest = top;
   bool again = !exact && !(top < INFINITY);  // selected again with scores in fp64: all of it
-  bool close = false;                        // ... only the order of the best
-  if (a.bias) {
+  if (BIAS) {
     largest = -INFINITY;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -643,7 +656,7 @@ __global__ void __launch_bounds__(kRouterThreads) router_rows_kernel(const __gri
 
   // values of 16 below the largest logit, of 2 below the largest s + bias,
   // share the lowest step: where that is chosen, the slow selection decides
-  const float scale = a.bias ? 0.5f : 0.0625f, steps = scale * float(1u << (31 - IB));
+  const float scale = BIAS ? 0.5f : 0.0625f, steps = scale * float(1u << (31 - IB));
   const float shift = __fmaf_rd(-largest, scale, 1.0f - 0x1p-22f);  // down: no value reaches 1
   uint32_t key[NC][8];
 #pragma unroll
@@ -704,7 +717,7 @@ __global__ void __launch_bounds__(kRouterThreads) router_rows_kernel(const __gri
     for (int c = 1; c < 7; ++c)
       if (a.topk_groups == c + 1) low = order[c], high = order[c + 1];
     // steps apart by which the order is certain: of sums of two rounded values
-    if (!exact) again |= float((low >> 3) - (high >> 3)) <= 2.0f * near * steps + (a.bias ? 2.0f : 0.0f);
+    if (!exact) again |= float((low >> 3) - (high >> 3)) <= 2.0f * near * steps + (BIAS ? 2.0f : 0.0f);
     kept = 0;
     bool mine = false;
     int g = a.groups, left = 0;
@@ -720,17 +733,19 @@ __global__ void __launch_bounds__(kRouterThreads) router_rows_kernel(const __gri
     }
   }
 
-  uint32_t out = 0;
+  uint32_t out = 0, out2 = 0;
 #pragma unroll
   for (int c = 1; c < NC; ++c)
-    if (c < chunks) merge_keys(key[0], key[c], out);
+    if (c < chunks) merge_keys<BIAS>(key[0], key[c], out, out2);
 #pragma unroll
   for (int o = 1; o < kRowLanes; o <<= 1) {
     uint32_t other[8];
 #pragma unroll
     for (int v = 0; v < 8; ++v) other[v] = __shfl_xor_sync(kFull, key[0][v], o);
-    out = max(out, __shfl_xor_sync(kFull, out, o));
-    merge_keys(key[0], other, out);
+    const uint32_t its = __shfl_xor_sync(kFull, out, o);
+    if (BIAS) out2 = max(min(out, its), max(out2, __shfl_xor_sync(kFull, out2, o)));
+    out = max(out, its);
+    merge_keys<BIAS>(key[0], other, out, out2);
   }
 
   // every lane of the token holds the list: through shared memory, two choices a lane
@@ -739,24 +754,62 @@ __global__ void __launch_bounds__(kRouterThreads) router_rows_kernel(const __gri
     *reinterpret_cast<uint4*>(list) = make_uint4(key[0][0], key[0][1], key[0][2], key[0][3]);
     *reinterpret_cast<uint4*>(list + 4) = make_uint4(key[0][4], key[0][5], key[0][6], key[0][7]);
     list[8] = out;
+    list[9] = out2;
   }
   __syncwarp();
+  auto index = [&](uint32_t key) { return exact ? int(0xFFFFu - (key & 0xFFFFu)) : int(kLast - (key & kLast)); };
+  // whether places q and q + 1 of the order may be the other way round
+  auto uncertain = [&](int q) {
+    const uint32_t mine = list[q], then = list[q + 1];
+    if (then == 0 || float((mine >> IB) - (then >> IB)) > near * steps + (BIAS ? 1.0f : 0.0f)) return false;
+    // the same logit and the same bias tie for certain, and stand in order of
+    // index; not so from the last choice on, where a later one may pass both
+    const int e = index(mine), f = index(then);
+    return q >= k - 1 || !(to_f32(row[e]) == to_f32(row[f]) && (!BIAS || a.bias[e] == a.bias[f]));
+  };
   int id[2];
+  unsigned pairs = 0;  // bit q: places q and q + 1 are uncertain
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int q = lane + i * kRowLanes;
-    const uint32_t mine = list[q], then = list[q + 1];
-    id[i] = q >= k ? 0 : exact ? int(0xFFFFu - (mine & 0xFFFFu)) : int(kLast - (mine & kLast));
-    if (!exact && q < k) {
-      again |= mine < kNoStep;
-      if (then != 0 && float((mine >> IB) - (then >> IB)) <= near * steps + (a.bias ? 1.0f : 0.0f)) {
-        // the same logit and the same bias tie for certain, and stand in order
-        // of index; not so for the last choice, where a later one may pass both
-        const int e = id[i], f = int(kLast - (then & kLast));
-        if (q == k - 1 || !(to_f32(row[e]) == to_f32(row[f]) && (!a.bias || a.bias[e] == a.bias[f]))) close = true;
-      }
+    id[i] = q >= k ? 0 : index(list[q]);
+    if (!exact) {
+      again |= q < k && list[q] < kNoStep;
+      if ((BIAS || q < k) && uncertain(q)) pairs |= 1u << q;
     }
     s_id[warp][sub][q] = id[i];
+  }
+  if (BIAS && lane == 0 && uncertain(8)) pairs |= 1u << 8;
+  const unsigned group_lanes = (1u << kRowLanes) - 1u;
+  bool close = !exact && (pairs & ((1u << k) - 1u)) != 0;
+  if (BIAS && a.sigmoid && __any_sync(kFull, close)) {
+    // the first `count` places hold what they should, in whatever order: settled among them, by every token at once
+#pragma unroll
+    for (int o = 1; o < kRowLanes; o <<= 1) pairs |= __shfl_xor_sync(kFull, pairs, o);
+    const int count = k + __ffs(~(pairs >> (k - 1))) - 1;
+    close = (pairs & ((1u << k) - 1u)) != 0;
+    const bool here = close && count <= 9;
+    double* value = reinterpret_cast<double*>(s_key[warp]) + sub * 12;
+    if (here) {
+#pragma unroll 1
+      for (int q = lane; q < count; q += kRowLanes) value[q] = sigmoid_f64(row, a.bias, index(list[q]));
+    }
+    __syncwarp();
+    if (here) {
+#pragma unroll 1
+      for (int q = lane; q < count; q += kRowLanes) {
+        const int e = index(list[q]);
+        const double x = value[q];
+        int rank = 0;
+#pragma unroll 1
+        for (int i = 0; i < count; ++i) rank += value[i] > x || (value[i] == x && index(list[i]) < e);
+        if (rank < k) s_id[warp][sub][rank] = e;
+      }
+      close = false;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) id[i] = lane + i * kRowLanes < k ? s_id[warp][sub][lane + i * kRowLanes] : 0;
   }
   const unsigned slow = __ballot_sync(kFull, again), any = slow | __ballot_sync(kFull, close);
   if (any) {
@@ -767,13 +820,13 @@ __global__ void __launch_bounds__(kRouterThreads) router_rows_kernel(const __gri
 #pragma unroll 1
     for (int i = 0; i < PER_WARP; ++i) {  // the whole warp, token after token
       const int lead = i * kRowLanes;
-      if (!(any >> lead & ((1u << kRowLanes) - 1u))) continue;
+      if (!(any >> lead & group_lanes)) continue;
       const int64_t t = __shfl_sync(kFull, r, lead);
       const T* its = static_cast<const T*>(a.z) + t * a.ld;
       const float its_from = __shfl_sync(kFull, from, lead), its_base = __shfl_sync(kFull, base, lead);
       const float its_inv = __shfl_sync(kFull, inv, lead);
       const uint32_t its_kept = __shfl_sync(kFull, kept, lead);
-      if ((slow >> lead & ((1u << kRowLanes) - 1u)) ||
+      if ((slow >> lead & group_lanes) ||
           !order_near<T>(a, its, its_from, its_kept, its_base, its_inv, a.groups > 1 ? a.per : 512,
                          reinterpret_cast<uint32_t*>(s_key[warp]), s_id[warp][i]))
         select_f64<T>(a, its, s_key[warp], s_id[warp][i]);
@@ -1038,7 +1091,9 @@ int launch_rows(RouterArgs& a, cudaStream_t s) {
   a.vec_bias = a.experts % 8 == 0 && aligned16(a.bias);
   a.cnt = a.per / 32;
   const int rows = kRouterThreads / kRowLanes;
-  router_rows_kernel<T, NC><<<unsigned((a.n + rows - 1) / rows), kRouterThreads, 0, s>>>(a);
+  const unsigned blocks = unsigned((a.n + rows - 1) / rows);
+  if (a.bias) router_rows_kernel<T, NC, true><<<blocks, kRouterThreads, 0, s>>>(a);
+  else router_rows_kernel<T, NC, false><<<blocks, kRouterThreads, 0, s>>>(a);
   return cuda_status(cudaGetLastError());
 }
 
