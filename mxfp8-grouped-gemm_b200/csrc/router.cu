@@ -402,9 +402,10 @@ __global__ void __launch_bounds__(kRouterThreads) router_topk_kernel(const __gri
     // argument), and 3 * 2^-24 s from the sum and the reciprocal: at most
     // 2^-24 s (7 + 1.5 |z|), which is largest for the largest s (and below
     // 2^-24 s 7 where z > 0); softmax has a sum of V + 5 roundings in place of
-    // 1 + exp, and |z| s is at most 0.37 of its largest s.  Twice that for a pair
+    // 1 + exp, and |z| s is at most 0.37 of its largest s.  Twice that for a
+    // pair, and what lies under 2^-126 and became 0
     const float big = a.sigmoid ? sigmoid_fast(top) : inv;
-    near = 0x1p-24f * big * (a.sigmoid ? 14.0f + 3.0f * fmaxf(0.0f, -top) : 2.0f * V + 40.0f);
+    near = 0x1p-24f * big * (a.sigmoid ? 14.0f + 3.0f * fmaxf(0.0f, -top) : 2.0f * V + 40.0f) + 0x1p-124f;
     again = a.sigmoid && top < -80.0f;                               // the scores vanish in fp32
   }
   if (a.bias) {

@@ -215,6 +215,21 @@ def test_rows_without_an_expert_go_by_the_bias(mxg, cuda_dev, E, n):
             _check(mxg, z, k, score=score, bias=bias)
 
 
+@pytest.mark.parametrize("E", [7, 24, 64, 256])
+@pytest.mark.parametrize("n", [40, 4200])
+def test_scores_at_the_end_of_the_range_of_fp32(mxg, cuda_dev, E, n):
+    """Scores and biases of about 1e-38 beside a larger one."""
+    g = torch.Generator(device=cuda_dev).manual_seed(E)
+    z = torch.rand(n, E, generator=g, device=cuda_dev) * 6 - 91
+    z[:, E // 2] = -79.0
+    bias = -torch.sigmoid(z[0].double()).float()
+    for k in (1, 4, 7):
+        _check(mxg, z, k, score="sigmoid", bias=bias)
+        _check(mxg, z + 79, k, score="softmax", bias=bias)
+        if E != 7:
+            _check(mxg, z, k, score="sigmoid", bias=bias, groups=8, topk_groups=5, group_score="top2")
+
+
 def test_nan_rows_have_ids_in_range(mxg, cuda_dev):
     z = _logits(6, 256, "fp32", 5, cuda_dev)
     z[0, 17] = z[1, :] = float("nan")
