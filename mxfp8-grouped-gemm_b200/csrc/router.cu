@@ -426,6 +426,7 @@ __global__ void __launch_bounds__(kRouterThreads) router_topk_kernel(const __gri
   for (int v = 0; v < V; v += 4)
     *reinterpret_cast<float4*>(list + lane * V + v) = make_float4(x[v], x[v + 1], x[v + 2], x[v + 3]);
   float head = x[0];
+  bool kept = true;                                                  // this lane's group
 
   if (G > 1) {
     // the two best of the group, over its lanes
@@ -447,7 +448,7 @@ __global__ void __launch_bounds__(kRouterThreads) router_topk_kernel(const __gri
       const float o = __shfl_sync(kFull, score, g << a.lpg_log2, LANES);
       better += o > score || (o == score && g < group);
     }
-    const bool kept = better < a.topk_groups && group < G;
+    kept = better < a.topk_groups && group < G;
     const float low = -lanes_max<LANES>(kept ? -score : -INFINITY), high = lanes_max<LANES>(kept ? -INFINITY : score);
     if (groups_scored) {
       // two sums of two, and their roundings
@@ -476,8 +477,6 @@ __global__ void __launch_bounds__(kRouterThreads) router_topk_kernel(const __gri
       head = code < V * 256 ? next[code >> 8] : -INFINITY;
     }
   }
-  // the best of what no round named: the order of the last choices is certain against it too
-  const float after = a.bias ? lanes_max<LANES>(head) : -INFINITY;
   __syncwarp();
   auto expert = [&](float2 c) {  // index of a choice
     const int l = __float_as_int(c.y) & 255;
@@ -496,6 +495,8 @@ __global__ void __launch_bounds__(kRouterThreads) router_topk_kernel(const __gri
     }
     return (l >> a.lpg_log2) * per + (l & ((1 << a.lpg_log2) - 1)) * a.cnt + at;
   };
+  auto apart = [&](float u, float v) { return u - v > near + 0x1p-23f * (fabsf(u) + fabsf(v)) || v == -INFINITY; };
+  bool tied = false;
   for (int q = lane; q < k; q += LANES) {
     const float2 c = rec[q];
     again |= c.x == -INFINITY;
@@ -503,13 +504,25 @@ __global__ void __launch_bounds__(kRouterThreads) router_topk_kernel(const __gri
     s_id[sub][q] = e;
     if (a.bias && q + 1 < rounds) {
       const float2 d = rec[q + 1];
-      auto apart = [&](float u, float v) { return u - v > near + 0x1p-23f * (fabsf(u) + fabsf(v)); };
       if (!apart(c.x, d.x)) {
-        // the same logit and the same bias tie for certain, and stand in order
-        // of index; the last choice only where what follows the two is apart
+        // the same logit and the same bias tie for certain, and stand in order of index
         const int j = expert(d);
-        if (!(to_f32(row[e]) == to_f32(row[j]) && a.bias[e] == a.bias[j])) again = true;
-        if (q == k - 1 && !apart(d.x, after)) again = true;
+        const bool same = to_f32(row[e]) == to_f32(row[j]) && a.bias[e] == a.bias[j];
+        again |= !same;
+        tied |= same && q == k - 1;
+      }
+    }
+  }
+  if (__any_sync(kFull, tied)) {
+    // equal to the last choice is the first left out: certain where all that follows as closely is equal too
+    __syncwarp();
+    const float last = rec[k - 1].x;
+    const int e = s_id[sub][k - 1];
+    if ((__ballot_sync(kFull, tied) & mask) && kept) {
+      for (int v = 0; v < have; ++v) {
+        const float c = vals[lane * V + v];
+        if (c > last || apart(last, c)) continue;
+        again |= !(to_f32(row[e]) == to_f32(row[first + v]) && a.bias[e] == a.bias[first + v]);
       }
     }
   }
