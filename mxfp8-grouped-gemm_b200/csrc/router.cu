@@ -772,36 +772,40 @@ __global__ void __launch_bounds__(kRouterThreads) router_rows_kernel(const __gri
   }
   __syncwarp();
   auto index = [&](uint32_t key) { return exact ? int(0xFFFFu - (key & 0xFFFFu)) : int(kLast - (key & kLast)); };
-  // whether places q and q + 1 of the order may be the other way round
-  auto uncertain = [&](int q) {
-    const uint32_t mine = list[q], then = list[q + 1];
-    if (then == 0 || float((mine >> IB) - (then >> IB)) > near * steps + (BIAS ? 1.0f : 0.0f)) return false;
-    // the same logit and the same bias tie for certain, and stand in order of
-    // index; not so from the last choice on, where a later one may pass both
-    const int e = index(mine), f = index(then);
-    return q >= k - 1 || !(to_f32(row[e]) == to_f32(row[f]) && (!BIAS || a.bias[e] == a.bias[f]));
-  };
   int id[2];
-  unsigned pairs = 0;  // bit q: places q and q + 1 are uncertain
+  unsigned pairs = 0;  // bit q: places q and q + 1 may be the other way round; bit 16 + q: and are not equal
+  auto look = [&](int q) {
+    const uint32_t mine = list[q], then = list[q + 1];
+    if (then == 0 || float((mine >> IB) - (then >> IB)) > near * steps + (BIAS ? 1.0f : 0.0f)) return;
+    // the same logit and the same bias tie for certain, and stand in order of index
+    const int e = index(mine), f = index(then);
+    const bool same = to_f32(row[e]) == to_f32(row[f]) && (!BIAS || a.bias[e] == a.bias[f]);
+    pairs |= (same ? 1u : 0x10001u) << q;
+  };
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int q = lane + i * kRowLanes;
     id[i] = q >= k ? 0 : index(list[q]);
     if (!exact) {
       again |= q < k && list[q] < kNoStep;
-      if ((BIAS || q < k) && uncertain(q)) pairs |= 1u << q;
+      look(q);
     }
     s_id[warp][sub][q] = id[i];
   }
-  if (BIAS && lane == 0 && uncertain(8)) pairs |= 1u << 8;
+  if (BIAS && lane == 0) look(8);
   const unsigned group_lanes = (1u << kRowLanes) - 1u;
-  bool close = !exact && (pairs & ((1u << k) - 1u)) != 0;
-  if (BIAS && a.sigmoid && __any_sync(kFull, close)) {
-    // the first `count` places hold what they should, in whatever order: settled among them, by every token at once
+  bool close = (pairs >> 16 & ((1u << k) - 1u)) || (pairs >> (k - 1) & 1u);
+  if (__any_sync(kFull, close)) {
+    // the first `count` places hold what they should: certain where those in doubt are equal
+    constexpr int MOST = BIAS ? 9 : 8;
 #pragma unroll
     for (int o = 1; o < kRowLanes; o <<= 1) pairs |= __shfl_xor_sync(kFull, pairs, o);
-    const int count = k + __ffs(~(pairs >> (k - 1))) - 1;
-    close = (pairs & ((1u << k) - 1u)) != 0;
+    const int count = k + __ffs(~(pairs >> (k - 1) & 0xFFFFu)) - 1;
+    close = count > MOST || (pairs >> 16 & ((1u << (count - 1)) - 1u));
+  }
+  if (BIAS && a.sigmoid && __any_sync(kFull, close)) {
+    // ... else settled among them, by every token at once
+    const int count = k + __ffs(~(pairs >> (k - 1) & 0xFFFFu)) - 1;
     const bool here = close && count <= 9;
     double* value = reinterpret_cast<double*>(s_key[warp]) + sub * 12;
     if (here) {
