@@ -549,11 +549,13 @@ __global__ void __launch_bounds__(kRouterThreads) router_topk_kernel(const __gri
 // (16-bit logits without a bias: the 16 bits themselves, exact).  Every chunk
 // is sorted in a lane, then the eight largest are merged over the chunks and
 // over the lanes.  Of what the merges leave out the largest is kept, and with a
-// bias the two largest: where the first places of these ten that hold all the
-// choices are apart from the rest, a token whose order is in doubt is settled
-// by its own lanes among them, which costs the throughput 5% and saves a warp
-// that is alone on its token at the end: 16384 rows of 256, sigmoid, bias,
-// groups 18.6 -> 15.9 us; bf16 with a bias of zero (ties) 19.8 -> 16.6 at 8192.
+// bias the two largest, which costs 5% of the throughput: where the first places
+// of these ten that hold all choices are apart from the rest, a token whose
+// order is in doubt is settled by its own lanes, and no warp is alone with it at
+// the end.  us before and after: 16384 rows of 256 with sigmoid, bias and groups
+// 18.8, 17.6 (16 to 19: what is left are groups in doubt, some in a call or
+// none); bf16 with a bias of zero (ties), 8192 rows, sigmoid 19.8, 14.4, softmax
+// 23.4, 15.9; without a bias, bf16 values in fp32, 13.0, 5.6.
 constexpr int kRowLanes = 4, kRowMost = 8;
 
 template <int A, int B>
@@ -802,6 +804,21 @@ __global__ void __launch_bounds__(kRouterThreads) router_rows_kernel(const __gri
     for (int o = 1; o < kRowLanes; o <<= 1) pairs |= __shfl_xor_sync(kFull, pairs, o);
     const int count = k + __ffs(~(pairs >> (k - 1) & 0xFFFFu)) - 1;
     close = count > MOST || (pairs >> 16 & ((1u << (count - 1)) - 1u));
+    const bool few = close && !(pairs >> 16 & ((1u << (k - 1)) - 1u));
+    if (!BIAS && __any_sync(kFull, few)) {
+      // only the last choice: certain where as many logits are above it as there are choices above it
+      const float last = to_f32(row[index(list[k - 1])]);
+      int above = 0;
+      if (few) {
+#pragma unroll 16
+        for (int e = lane; e < E; e += kRowLanes)
+          above += to_f32(row[e]) > last && (a.groups == 1 || (kept >> (e / a.per) & 1u));
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) above -= lane + i * kRowLanes < k && to_f32(row[id[i]]) > last;
+      above = lanes_sum<kRowLanes>(above);
+      if (few && above == 0) close = false;
+    }
   }
   if (BIAS && a.sigmoid && __any_sync(kFull, close)) {
     // ... else settled among them, by every token at once

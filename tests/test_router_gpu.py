@@ -152,6 +152,19 @@ def test_equal_experts_at_the_last_choice(mxg, cuda_dev, E, n):
             _check(mxg, near, k, score="sigmoid", bias=bias, groups=8, topk_groups=8)
 
 
+@pytest.mark.parametrize("E", [40, 256, 384])
+@pytest.mark.parametrize("n", [70, 8203])
+def test_many_ties(mxg, cuda_dev, E, n):
+    """Logits of few digits in every type, and a bias of zero."""
+    zero = torch.zeros(E, device=cuda_dev)
+    for dtype in DT.values():
+        z = _logits(n, E, "bf16", E, cuda_dev).to(dtype)
+        _check(mxg, z, 8)
+        _check(mxg, z, 3, groups=2, topk_groups=1)
+        for score in ("softmax", "sigmoid"):
+            _check(mxg, z, 8, score=score, bias=zero)
+
+
 @pytest.mark.parametrize("E", [16, 40, 256, 384])
 @pytest.mark.parametrize("n", [20, 8200])
 def test_logits_and_biases_far_from_zero(mxg, cuda_dev, E, n):
