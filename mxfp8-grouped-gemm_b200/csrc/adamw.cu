@@ -205,8 +205,8 @@ __device__ __forceinline__ float rcp_fast(float x) {
 }
 
 struct StepConsts {
-  float lr;
-  float rs2, eps;  // -1 / sqrt(1 - b2^t) and -eps, over lr / (1 - b1^t): m / (sqrt(v) rs2 + eps) is the step
+  float size, rs2;   // -lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+  const float* bc1;  // 1 - b1^t, in shared memory: registers are short
   uint32_t key;
 };
 
@@ -249,11 +249,12 @@ __device__ __forceinline__ void update(const AdamArgs& a, const StepConsts& k, f
     split(mul(mul(gg, gg), both(a.c2)), d0, d1);
     split(mul(two(v[i], v[i + 1]), both(a.b2)), v[i], v[i + 1]);
     v[i] = __fadd_rn(v[i], d0), v[i + 1] = __fadd_rn(v[i + 1], d1);
-    split(fma2(two(sqrt_fast(v[i]), sqrt_fast(v[i + 1])), both(k.rs2), both(k.eps)), d0, d1);
-    // the decay joins the update: one rounding of the weight's size
+    split(fma2(two(sqrt_fast(v[i]), sqrt_fast(v[i + 1])), both(k.rs2), both(a.eps)), d0, d1);
+    // lr is a factor of what is finite, last of all, so that with lr 0 the weight stays whatever v is; the
+    // decay joins the update: one rounding of the weight's size
     const Two by = mul(two(m[i], m[i + 1]), two(rcp_fast(d0), rcp_fast(d1)));
-    split(fma2(two(p[i], p[i + 1]), both(decay), by), d0, d1);
-    p[i] += d0, p[i + 1] += d1;
+    const Two old = two(p[i], p[i + 1]);
+    split(fma2(fma2(old, both(decay), by), both(k.size), old), p[i], p[i + 1]);
   }
   float im = 0.0f, iv = 0.0f, rm[2], rv[2];
   if constexpr (BITS == 32) {
@@ -309,7 +310,7 @@ __device__ __forceinline__ void adamw_chunk(const AdamArgs& a, const StepConsts&
   using S = typename B::S;
   constexpr uint32_t kStep = kAdamThreads * 8;
   const uint32_t lane = threadIdx.x & 31;
-  const float decay = -k.lr * t.weight_decay;
+  const float decay = *k.bc1 * t.weight_decay;  // over -lr / (1 - b1^t), as the update is
   const int64_t at = t.offset + i0;
   P* param = static_cast<P*>(t.param) + i0;
   const G* grad = reinterpret_cast<const G*>(g) + i0;
@@ -399,10 +400,9 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const __grid_consta
   if (threadIdx.x == 32) s_bc[1] = float(-expm1(double(t) * a.ln_b2));
   __syncthreads();
   StepConsts k;
-  k.lr = a.lr_ptr ? *a.lr_ptr : a.lr;
-  const float size = -k.lr / s_bc[0];  // lr 0: both infinite, and the step 0
-  k.rs2 = 1.0f / (sqrtf(s_bc[1]) * size);
-  k.eps = a.eps / size;
+  k.bc1 = s_bc;
+  k.size = -(a.lr_ptr ? *a.lr_ptr : a.lr) / s_bc[0];
+  k.rs2 = 1.0f / sqrtf(s_bc[1]);
   k.key = step_key(a.seed_lo, a.seed_hi, uint32_t(t));
   int64_t c = blockIdx.x;
   int ti = c < a.n_chunks ? a.chunks[a.chunk0 + c] : 0;

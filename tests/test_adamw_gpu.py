@@ -302,3 +302,37 @@ def test_elements_past_32_bits(mxg, cuda_dev):
     assert 0 < float((p != 0.5).float().mean()) and torch.all((p - 0.5).abs() <= 2.0 ** -8)
     del p, g, opt
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("master", [True, False])
+@pytest.mark.parametrize("lr", [0.0, 1e-42])
+def test_lr_zero_leaves_every_weight(mxg, cuda_dev, bits, master, lr):
+    """A warm-up's first step, with second moments of 0 and under fp32's normal
+    range among others.  1e-42: an update of at most 10 * lr, under half a
+    step of any weight here."""
+    shapes, dtypes = [(700,), (513,), (300,)], [BF, F32, BF]
+    for as_tensor in (False, True):
+        params = [p.add_(1.0) for p in _make(shapes, dtypes, 40, cuda_dev)]
+        before = [p.clone() for p in params]
+        opt = mxg.optim.AdamW(params, state_bits=bits, master_weights=master, weight_decay=0.1,
+                              lr=torch.full((1,), lr, device=cuda_dev) if as_tensor else lr)
+        grads = _make(shapes, [F32, BF, BF], 41, cuda_dev)
+        grads[0][::2] = 0
+        grads[0][1::4] = 1e-25
+        grads[1].zero_()
+        grads[2][:256] = 1e-25
+        for _ in range(2):
+            opt.step(grads)
+        assert all(torch.equal(p, b) for p, b in zip(params, before))
+        if opt.master is not None:
+            assert torch.equal(opt.master[:700], before[0].float())
+        # and the run goes on from there
+        if as_tensor:
+            opt.lr.fill_(1e-3)
+        else:
+            opt.lr = 1e-3
+        opt.step(grads)
+        assert all(torch.isfinite(p).all() for p in params)
+        decayed = before[1].double() * (1 - 1e-4)
+        assert torch.all((params[1].double() - decayed).abs() <= 2.0 ** -22 * decayed)
