@@ -193,9 +193,12 @@ __device__ __forceinline__ float as_f32(__nv_bfloat16 x) { return __bfloat162flo
 __device__ __forceinline__ void put(float* p, float x) { *p = x; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
+// SMALL: an x under 2^-126 has a root too, else it counts as 0.
+template <bool SMALL>
 __device__ __forceinline__ float sqrt_fast(float x) {
   float y;
-  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  if constexpr (SMALL) asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  else asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 __device__ __forceinline__ float rcp_fast(float x) {
@@ -222,7 +225,7 @@ struct Block {
 };
 
 // The update of one block, in place; block: its number in the moments.
-template <typename P, typename G, bool MASTER, int BITS>
+template <typename P, typename G, bool MASTER, int BITS, bool SMALL>
 __device__ __forceinline__ void update(const AdamArgs& a, const StepConsts& k, float decay, uint64_t block, int lane,
                                        Block<P, G, MASTER, BITS>& x) {
   constexpr bool kStochastic = !MASTER && sizeof(P) == 2;
@@ -237,7 +240,7 @@ __device__ __forceinline__ void update(const AdamArgs& a, const StepConsts& k, f
     decode_v(x.v.w[0], x.sv, v, 0), decode_v(x.v.w[1], x.sv, v, 4);
   }
   // the update alone goes through the approximate root and reciprocal (2 units
-  // of the last place; a v under 2^-126 counts as 0 beside eps)
+  // of the last place)
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
     const Two gg = two(g[i], g[i + 1]);
@@ -249,7 +252,7 @@ __device__ __forceinline__ void update(const AdamArgs& a, const StepConsts& k, f
     split(mul(mul(gg, gg), both(a.c2)), d0, d1);
     split(mul(two(v[i], v[i + 1]), both(a.b2)), v[i], v[i + 1]);
     v[i] = __fadd_rn(v[i], d0), v[i + 1] = __fadd_rn(v[i + 1], d1);
-    split(fma2(two(sqrt_fast(v[i]), sqrt_fast(v[i + 1])), both(k.rs2), both(a.eps)), d0, d1);
+    split(fma2(two(sqrt_fast<SMALL>(v[i]), sqrt_fast<SMALL>(v[i + 1])), both(k.rs2), both(a.eps)), d0, d1);
     // lr is a factor of what is finite, last of all, so that with lr 0 the weight stays whatever v is; the
     // decay joins the update: one rounding of the weight's size
     const Two by = mul(two(m[i], m[i + 1]), two(rcp_fast(d0), rcp_fast(d1)));
@@ -303,7 +306,7 @@ __device__ __forceinline__ void update(const AdamArgs& a, const StepConsts& k, f
 // cache (352 M weights, blocks of 256 threads: 979 -> 935 us; through shared
 // memory instead 957, into registers 1265).  Addresses are those of the chunk, the same for
 // the whole block, plus a 32-bit offset.
-template <typename P, typename G, bool MASTER, int BITS>
+template <typename P, typename G, bool MASTER, int BITS, bool SMALL>
 __device__ __forceinline__ void adamw_chunk(const AdamArgs& a, const StepConsts& k, const mxg_adamw_tensor& t,
                                             uint64_t g, int64_t i0, int n) {
   using B = Block<P, G, MASTER, BITS>;
@@ -361,7 +364,7 @@ __device__ __forceinline__ void adamw_chunk(const AdamArgs& a, const StepConsts&
       fetch(v + o, x.v);
       if constexpr (BITS == 8) x.sm = ms[o >> 8], x.sv = vs[o >> 8];
     }
-    update(a, k, decay, block + (o >> 8), lane, x);
+    update<P, G, MASTER, BITS, SMALL>(a, k, decay, block + (o >> 8), lane, x);
     keep_words(m + o, x.m);
     keep_words(v + o, x.v);
     if (BITS == 8 && lane == 0) ms[o >> 8] = x.sm, vs[o >> 8] = x.sv;
@@ -391,7 +394,7 @@ __device__ __forceinline__ void adamw_chunk(const AdamArgs& a, const StepConsts&
   }
 }
 
-template <int BITS>
+template <int BITS, bool SMALL>
 __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const __grid_constant__ AdamArgs a) {
   __shared__ float s_bc[2];
   const int64_t t = *a.step + 1;
@@ -417,16 +420,16 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const __grid_consta
     const bool f32 = tagged & kGradF32;
     switch (T.kind) {
       case MXG_ADAMW_F32:
-        if (f32) adamw_chunk<float, float, false, BITS>(a, k, T, g, i0, n);
-        else adamw_chunk<float, __nv_bfloat16, false, BITS>(a, k, T, g, i0, n);
+        if (f32) adamw_chunk<float, float, false, BITS, SMALL>(a, k, T, g, i0, n);
+        else adamw_chunk<float, __nv_bfloat16, false, BITS, SMALL>(a, k, T, g, i0, n);
         break;
       case MXG_ADAMW_BF16_MASTER:
-        if (f32) adamw_chunk<__nv_bfloat16, float, true, BITS>(a, k, T, g, i0, n);
-        else adamw_chunk<__nv_bfloat16, __nv_bfloat16, true, BITS>(a, k, T, g, i0, n);
+        if (f32) adamw_chunk<__nv_bfloat16, float, true, BITS, SMALL>(a, k, T, g, i0, n);
+        else adamw_chunk<__nv_bfloat16, __nv_bfloat16, true, BITS, SMALL>(a, k, T, g, i0, n);
         break;
       default:
-        if (f32) adamw_chunk<__nv_bfloat16, float, false, BITS>(a, k, T, g, i0, n);
-        else adamw_chunk<__nv_bfloat16, __nv_bfloat16, false, BITS>(a, k, T, g, i0, n);
+        if (f32) adamw_chunk<__nv_bfloat16, float, false, BITS, SMALL>(a, k, T, g, i0, n);
+        else adamw_chunk<__nv_bfloat16, __nv_bfloat16, false, BITS, SMALL>(a, k, T, g, i0, n);
     }
   }
   // every block has read the step by the time the last one is done
@@ -500,7 +503,11 @@ extern "C" int mxg_adamw_step(const mxg_adamw_args* args, void* stream) {
   a.ln_b1 = std::log(r.beta1), a.ln_b2 = std::log(r.beta2);
   a.seed_lo = uint32_t(r.seed), a.seed_hi = uint32_t(r.seed >> 32);
   int per_sm = 0;
-  auto* kernel = state_bits == 8 ? adamw_kernel<8> : adamw_kernel<32>;
+  // The root of a second moment under 2^-126 is at most 2^-63, over sqrt(1 - b2) in the first step: from eps =
+  // 2^24 times that on it is lost in fp32's rounding.  Below, 8-bit states take the root with subnormals too (352 M
+  // weights: 1008 us for 987; 32-bit states, bound by HBM, take it always: 1626, 1624).
+  const bool small = state_bits == 32 || r.eps * std::sqrt(1.0 - r.beta2) < 0x1p-39;
+  auto* kernel = state_bits == 32 ? adamw_kernel<32, true> : small ? adamw_kernel<8, true> : adamw_kernel<8, false>;
   if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kAdamThreads, 0) != cudaSuccess || per_sm < 1)
     return MXG_ERR_CUDA;
   for (int t0 = 0; t0 < n_tensors; t0 += kAdamTensors) {

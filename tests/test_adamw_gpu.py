@@ -336,3 +336,22 @@ def test_lr_zero_leaves_every_weight(mxg, cuda_dev, bits, master, lr):
         assert all(torch.isfinite(p).all() for p in params)
         decayed = before[1].double() * (1 - 1e-4)
         assert torch.all((params[1].double() - decayed).abs() <= 2.0 ** -22 * decayed)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps", [1e-8, 1e-12, 1e-18, 1e-30])
+def test_second_moments_under_the_normal_range(mxg, cuda_dev, bits, eps):
+    """Gradients whose squares are subnormal or vanish beside an eps of any
+    size: the head's tolerance holds (the root has 2 units of the last place
+    there too)."""
+    params = [p.mul_(50) for p in _make([(1024,), (700,)], [F32, BF], 42, cuda_dev)]
+    mirror = Mirror(mxg.optim.AdamW(params, state_bits=bits, eps=eps, betas=(0.9, 0.999)))
+    for t in range(2):
+        grads = _make([(1024,), (700,)], [F32, BF], 43 + t, cuda_dev)
+        for g in grads:
+            g[:256] *= 1e-16                     # g^2 (1 - b2) of about 1e-38
+            g[256:512] *= 1e-18
+            g[512:600] *= 1e-21                  # vanishes
+            g[600:] *= 1e-17
+        mirror.step(grads)
+    assert all(torch.isfinite(p).all() for p in params)
