@@ -335,7 +335,7 @@ MXG_API int mxg_router_topk_bwd(const mxg_router_args* args, void* stream);
 /* ---- AdamW over many tensors in one launch ----
  * Moments are flat arrays in which tensor i starts at element offset[i], a
  * multiple of MXG_ADAMW_BLOCK; gaps hold zeros.  With g the gradient, t the
- * step (counted from 1), eps > 0 and every operation in f32:
+ * step (counted from 1), eps > 0 (a normal f32) and every operation in f32:
  *   m = b1 m + (1-b1) g,  v = b2 v + (1-b2) g^2,
  *   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps).
  * state_bits 32: moments are f32.  state_bits 8: a byte a value and an f32

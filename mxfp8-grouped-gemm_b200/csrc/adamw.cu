@@ -11,6 +11,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -483,7 +484,8 @@ extern "C" int mxg_adamw_step(const mxg_adamw_args* args, void* stream) {
     return MXG_ERR_INVALID_ARGUMENT;
   if (r.chunk < MXG_ADAMW_BLOCK || r.chunk % MXG_ADAMW_BLOCK || r.chunk > (1 << 24)) return MXG_ERR_INVALID_ARGUMENT;
   if (state_bits == 8 && (!r.exp_avg_scale || !r.exp_avg_sq_scale)) return MXG_ERR_INVALID_ARGUMENT;
-  if (!(r.lr >= 0.0) || !(r.beta1 >= 0.0 && r.beta1 < 1.0) || !(r.beta2 >= 0.0 && r.beta2 < 1.0) || !(r.eps > 0.0))
+  if (!(r.lr >= 0.0 && r.lr <= FLT_MAX) || !(r.beta1 >= 0.0 && r.beta1 < 1.0) ||
+      !(r.beta2 >= 0.0 && r.beta2 < 1.0) || !(r.eps >= FLT_MIN && r.eps <= FLT_MAX))
     return MXG_ERR_INVALID_ARGUMENT;
   for (int i = 0; i < n_tensors; ++i) {
     if (chunk_begin[i] < 0 || chunk_begin[i + 1] < chunk_begin[i]) return MXG_ERR_INVALID_ARGUMENT;

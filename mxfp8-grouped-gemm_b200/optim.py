@@ -12,6 +12,7 @@ import torch
 from . import _lib
 
 _GRAD = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
+_F32 = torch.finfo(torch.float32)
 _ENTRY = np.dtype([("param", "<u8"), ("numel", "<i8"), ("offset", "<i8"), ("master", "<i8"), ("decay", "<f4"),
                    ("kind", "<i4"), ("first_chunk", "<i8")])     # mxg_adamw_tensor
 
@@ -59,8 +60,8 @@ class AdamW:
             raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
         if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
             raise ValueError(f"betas must lie in [0, 1), got {betas}")
-        if not eps > 0.0:
-            raise ValueError(f"eps must be positive, got {eps}")
+        if not _F32.tiny <= eps <= _F32.max:
+            raise ValueError(f"eps must be positive and a normal fp32 number, got {eps}")
         decay = self._decays(weight_decay, len(params))
         for i, p in enumerate(params):
             if p.dtype not in _GRAD:
@@ -118,8 +119,8 @@ class AdamW:
         decay = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * count
         if len(decay) != count:
             raise ValueError(f"{len(decay)} weight decays for {count} tensors")
-        if not all(d >= 0.0 for d in decay):
-            raise ValueError("weight_decay must not be negative")
+        if not all(0.0 <= d <= _F32.max for d in decay):
+            raise ValueError("weight_decay must not be negative, nor beyond fp32's range")
         return decay
 
     def _lay_out(self):
@@ -153,8 +154,8 @@ class AdamW:
             if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != self.device:
                 raise ValueError(f"lr must be a number or a one-element fp32 tensor on {self.device}")
             lr, lr_ptr = 0.0, lr.data_ptr()
-        elif not 0.0 <= lr < float("inf"):
-            raise ValueError(f"lr must not be negative, got {lr}")
+        elif not 0.0 <= lr <= _F32.max:
+            raise ValueError(f"lr must not be negative, nor beyond fp32's range, got {lr}")
         held = None                                # contiguous copies, until the launch
         # all at once where every gradient is as it should be
         types = self._types(grads)

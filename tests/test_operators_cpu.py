@@ -166,3 +166,20 @@ def test_every_code_is_kept_by_a_round_trip():
         x[:kept.size] = ao.decode(np.resize(kept, 256), scale, first)[:kept.size]
         again, s = ao.encode(x, np.zeros(256, np.uint64), first)
         assert s[0] == 1.0 and np.array_equal(ao.decode(again, s, first)[:kept.size], x[:kept.size])
+
+
+def test_adamw_refuses_settings_beyond_fp32(mxg):
+    """An eps that fp32 holds as 0 or as a subnormal (0 / eps has no value
+    there), an lr or a decay that it holds as infinity."""
+    A, p, inf = mxg.optim.AdamW, torch.zeros(8), float("inf")
+    for eps in (1e-50, 1e-39, inf, float("nan")):
+        with pytest.raises(ValueError, match="eps"):
+            A([p], eps=eps)
+    for decay in (inf, 1e39, [1e39], float("nan")):
+        with pytest.raises(ValueError, match="decay"):
+            A([p], weight_decay=decay)
+    begin, grads, kinds = np.zeros(2, np.int64), np.array([16], np.uint64), np.array([1], np.int32)
+    for lr, eps in ((1e39, 1e-8), (inf, 1e-8), (1e-3, 1e-50), (1e-3, 1e-39), (1e-3, inf)):
+        assert mxg._lib.load().mxg_adamw_step(mxg._lib.adamw_args(
+            16, 16, begin.ctypes.data, grads.ctypes.data, kinds.ctypes.data, 16, 16, 0, 0, 0, 16, 16, 0, lr, 0.9,
+            0.99, eps, 0, 1, 4096, 32, 0), None) == 1
