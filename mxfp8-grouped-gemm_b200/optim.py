@@ -48,7 +48,9 @@ class AdamW:
     device, so a captured ``step`` counts on at every replay; ``lr`` may be a
     number (fixed at capture) or a one-element fp32 CUDA tensor that is read
     at every step.  ``lr``, ``betas``, ``eps`` and ``weight_decay`` may be set
-    between steps.  One optimiser's steps run one after the other: do not
+    between steps; a graph captured before keeps its ``betas``, ``eps``, number
+    ``lr`` and gradients' addresses, and from the next ``step`` call on takes
+    over a new ``weight_decay`` and the addresses of tensors that have moved.  One optimiser's steps run one after the other: do not
     issue them on several streams at once."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay=0.01, *,
@@ -102,6 +104,7 @@ class AdamW:
                 for p, at in zip(params, self._copies):
                     if at >= 0:
                         self.master[at:at + p.numel()].copy_(p.detach().reshape(-1))
+        self._table = torch.empty(len(params) * _ENTRY.itemsize, dtype=torch.uint8, device=dev)
         self._step = torch.zeros(1, dtype=torch.int64, device=dev)
         self._done = torch.zeros(1, dtype=torch.int32, device=dev)
         # What a thread block takes at a time: about 128 shares, long runs where there is much.  us of a bf16 step
@@ -124,7 +127,8 @@ class AdamW:
         return decay
 
     def _lay_out(self):
-        """The device table of the tensors (again when one has moved, or a weight decay changed)."""
+        """The device table of the tensors (again when one has moved, or a weight decay changed).  It stays where
+        it is: a captured step reads it at every replay."""
         self.weight_decay = self._decays(self.weight_decay, len(self.params))
         for i, (p, shape) in enumerate(zip(self.params, self._shapes)):
             if p.shape != shape or p.dtype != self._dtypes[i] or p.device != self.device or not p.is_contiguous():
@@ -137,7 +141,7 @@ class AdamW:
         t["decay"], t["first_chunk"] = self.weight_decay, self._chunk_begin[:-1]
         t["kind"] = [_lib.ADAMW_F32 if p.dtype == torch.float32 else
                      _lib.ADAMW_BF16_MASTER if c >= 0 else _lib.ADAMW_BF16 for p, c in zip(self.params, self._copies)]
-        self._table = torch.from_numpy(t.view(np.uint8)).to(self.device)
+        self._table.copy_(torch.from_numpy(t.view(np.uint8)))
         self._laid_out = list(self.weight_decay)
 
     def step(self, grads=None) -> None:

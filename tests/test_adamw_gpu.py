@@ -355,3 +355,38 @@ def test_second_moments_under_the_normal_range(mxg, cuda_dev, bits, eps):
             g[600:] *= 1e-17
         mirror.step(grads)
     assert all(torch.isfinite(p).all() for p in params)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_step_outlives_a_new_layout(mxg, cuda_dev, bits):
+    """A graph's table of tensors is the optimiser's: an eager step with another
+    weight decay, or after a tensor has moved, changes it in place."""
+    shapes, dtypes = [(5000,), (77, 3)], [BF, F32]
+    make = lambda: _make(shapes, dtypes, 50, cuda_dev)
+    a, b = make(), make()
+    grads = _make(shapes, [F32, F32], 51, cuda_dev, std=1e-3)
+    eager = mxg.optim.AdamW(a, state_bits=bits, weight_decay=0.1)
+    other = mxg.optim.AdamW(b, state_bits=bits, weight_decay=0.1)
+    table = other._table.data_ptr()
+    eager.step(grads), other.step(grads)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        other.step(grads)
+    graph.replay(), eager.step(grads)
+    for opt in (eager, other):
+        opt.weight_decay = 0.5
+        opt.step(grads)
+    assert other._table.data_ptr() == table
+    held = [torch.full((64,), 255, dtype=torch.uint8, device=cuda_dev) for _ in range(64)]   # what is freed, is reused
+    graph.replay(), eager.step(grads)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    old = b[0].data
+    b[0].data = old.clone()
+    keep = old.clone()
+    eager.step(grads), other.step(grads)
+    assert other._table.data_ptr() == table
+    graph.replay(), eager.step(grads)
+    assert all(torch.equal(x, y) for x, y in zip(a, b)) and torch.equal(old, keep)
+    assert torch.equal(eager.exp_avg, other.exp_avg) and torch.equal(eager.exp_avg_sq, other.exp_avg_sq)
+    assert eager.state_dict()["step"] == other.state_dict()["step"] == 6     # step, replay, step, replay, step, replay
+    del held
