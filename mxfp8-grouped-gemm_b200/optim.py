@@ -134,6 +134,8 @@ class AdamW:
             if p.shape != shape or p.dtype != self._dtypes[i] or p.device != self.device or not p.is_contiguous():
                 raise ValueError(f"params[{i}] is no longer a contiguous {tuple(shape)} {self._dtypes[i]} tensor on "
                                  f"{self.device}")
+            if p.numel() and p.data_ptr() == 0:
+                raise ValueError(f"params[{i}] has no memory")
         self._at = [p.data_ptr() for p in self.params]
         t = np.zeros(len(self.params), _ENTRY)
         t["param"], t["numel"] = self._at, [p.numel() for p in self.params]
@@ -162,14 +164,15 @@ class AdamW:
             raise ValueError(f"lr must not be negative, nor beyond fp32's range, got {lr}")
         held = None                                # contiguous copies, until the launch
         # all at once where every gradient is as it should be
-        types = self._types(grads)
-        if (None in types or [g.shape for g in grads] != self._shapes
-                or set(map(_get_device, grads)) != self._on or not all(map(_is_contiguous, grads))):
+        types, ptrs = self._types(grads), None
+        if (None not in types and [g.shape for g in grads] == self._shapes
+                and set(map(_get_device, grads)) == self._on and all(map(_is_contiguous, grads))):
+            ptrs = list(map(_data_ptr, grads))
+        if ptrs is None or 0 in ptrs:
             grads = held = self._checked(grads)
-            types = self._types(grads)
-        kinds = np.array([t or 0 for t in types] if held else types, np.int32)
-        ptrs = np.array([0 if g is None else g.data_ptr() for g in grads] if held else list(map(_data_ptr, grads)),
-                        np.uint64)
+            types = [t or 0 for t in self._types(grads)]
+            ptrs = [0 if g is None else g.data_ptr() for g in grads]
+        kinds, ptrs = np.array(types, np.int32), np.array(ptrs, np.uint64)
         if list(map(_data_ptr, params)) != self._at or self.weight_decay != self._laid_out:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("a tensor moved, or a weight decay changed, since the last step: take one step "
@@ -200,6 +203,8 @@ class AdamW:
                 if g.shape != shape or g.device != self.device:
                     raise ValueError(f"grads[{i}] is {tuple(g.shape)} on {g.device}, expected {tuple(shape)} on "
                                      f"{self.device}")
+                if g.numel() and g.data_ptr() == 0:
+                    raise ValueError(f"grads[{i}] has no memory")
                 g = g.contiguous()
             out.append(g)
         return out

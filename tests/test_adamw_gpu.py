@@ -390,3 +390,20 @@ def test_captured_step_outlives_a_new_layout(mxg, cuda_dev, bits):
     assert torch.equal(eager.exp_avg, other.exp_avg) and torch.equal(eager.exp_avg_sq, other.exp_avg_sq)
     assert eager.state_dict()["step"] == other.state_dict()["step"] == 6     # step, replay, step, replay, step, replay
     del held
+
+
+def test_tensors_without_memory_are_refused(mxg, cuda_dev):
+    """A weight or gradient whose storage was given back (sharded training does
+    that): no step, and the optimiser goes on once it is there again."""
+    p, g = _make([(300,), (40,)], [F32, BF], 60, cuda_dev), _make([(300,), (40,)], [F32, BF], 61, cuda_dev)
+    opt = mxg.optim.AdamW(p)
+    for t, name in ((g[1], "grads"), (p[0], "params")):
+        keep = t.clone()
+        t.untyped_storage().resize_(0)
+        with pytest.raises(ValueError, match=rf"{name}\[\d\] has no memory"):
+            opt.step(g)
+        t.untyped_storage().resize_(keep.numel() * keep.element_size())
+        t.copy_(keep)
+    assert opt.state_dict()["step"] == 0
+    opt.step(g)
+    assert opt.state_dict()["step"] == 1 and mxg.device_error() == 0
