@@ -319,7 +319,7 @@ __device__ __forceinline__ void write_weights(const RouterArgs& a, const T* row,
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
-      float p = __expf(y[i] - (a.sigmoid && y[i] > 0.0f ? y[i] : shift));
+      float p = __expf(a.sigmoid && y[i] > 0.0f ? 0.0f : y[i] - shift);
       if (a.sigmoid) p = __fdividef(p, 1.0f + __expf(-fabsf(y[i])));
       y[i] = y[i] == -INFINITY ? 0.0f : p;
       sum += y[i];

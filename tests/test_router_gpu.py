@@ -500,3 +500,25 @@ def test_captured_backward_pass(mxg, cuda_dev):
     want = both()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert mxg.device_error() == 0
+
+
+@pytest.mark.parametrize("E,k", [(8, 2), (16, 16), (64, 4), (256, 8), (384, 12)])
+@pytest.mark.parametrize("n", [5, 8200])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_sigmoid_of_infinite_logits(mxg, cuda_dev, E, k, n, dtype):
+    """sigmoid(inf) is 1, in a share too: weights and gradients are finite."""
+    inf = float("inf")
+    z = _logits(n, E, dtype, 7, cuda_dev)
+    z[0, E // 2] = inf
+    z[1, ::2] = inf
+    z[2] = inf
+    z[3] = -inf
+    z[3, 1] = inf
+    bias = torch.randn(E, device=cuda_dev, generator=torch.Generator(cuda_dev).manual_seed(E)) * 0.05
+    for renorm in (True, False):
+        for b in (None, bias):
+            w, ids = _check(mxg, z, k, score="sigmoid", bias=b, renormalize=renorm, scale=2.5)
+            assert torch.isfinite(w).all()
+        dw = torch.randn(n, k, device=cuda_dev, generator=torch.Generator(cuda_dev).manual_seed(8))
+        dz = mxg.ops.router_topk_bwd(z, w, ids, dw, score="sigmoid", renormalize=renorm, scale=2.5)
+        assert torch.isfinite(dz).all() and torch.all(dz[z == inf] == 0)
