@@ -522,3 +522,30 @@ def test_sigmoid_of_infinite_logits(mxg, cuda_dev, E, k, n, dtype):
         dw = torch.randn(n, k, device=cuda_dev, generator=torch.Generator(cuda_dev).manual_seed(8))
         dz = mxg.ops.router_topk_bwd(z, w, ids, dw, score="sigmoid", renormalize=renorm, scale=2.5)
         assert torch.isfinite(dz).all() and torch.all(dz[z == inf] == 0)
+
+
+@pytest.mark.parametrize("E", [8, 30, 64, 137, 256, 384])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_dense_gradient_of_logits_far_from_zero(mxg, cuda_dev, E, dtype):
+    """Softmax, not renormalised, at offsets up to the end of the type's range
+    (the logits that are left of them, the oracle takes as they are)."""
+    top = torch.finfo(DT[dtype]).max
+    z = _logits(14, E, "fp32", 11, cuda_dev)
+    for r, off in enumerate((-1e4, 300.0, 5e5, -7.3e5, 1e6, -3e6, 3e9, 1e30, -1e30, 3e38, -3e38)):
+        z[r] += off
+    z[11] = -top                                 # the lowest value throughout
+    z[12] = top
+    z[13] = -top
+    z[13, 3] = -float("inf")
+    z[13, 5] = top
+    z[0, 1] = z[7, 2] = -float("inf")
+    z = z.clamp(-top, top).where(z != -float("inf"), z).to(DT[dtype])
+    k = min(E, 6)
+    w, ids = mxg.ops.router_topk(z, k, renormalize=False, scale=2.5)
+    dw = torch.randn(14, k, device=cuda_dev, generator=torch.Generator(cuda_dev).manual_seed(1))
+    dz = mxg.ops.router_topk_bwd(z, w, ids, dw, renormalize=False, scale=2.5)
+    ref = ro.router_bwd(_np(z), ids.cpu().numpy(), _np(dw), renormalize=False, scale=2.5)
+    size = np.abs(_np(w) * _np(dw)).sum(1, keepdims=True)
+    half = 0.0 if dtype == "fp32" else torch.finfo(DT[dtype]).eps / 2
+    assert np.all(np.abs(_np(dz) - ref) <= G_TOL * size + half * np.abs(ref) + 1e-37)
+    assert mxg.device_error() == 0
