@@ -209,7 +209,8 @@ __device__ __noinline__ void select_f64(const RouterArgs& a, const T* row, uint6
       b2 = fmax(fmin(b1, o1), fmax(b2, o2));
       b1 = fmax(b1, o1);
     }
-    const double score = a.top2 && a.per > 1 ? b1 + b2 : b1;
+    double score = a.top2 && a.per > 1 ? b1 + b2 : b1;
+    if (score != score) score = -INFINITY;  // inf - inf
     int better = 0;
 #pragma unroll 4
     for (int g = 0; g < a.groups; ++g) {

@@ -549,3 +549,27 @@ def test_dense_gradient_of_logits_far_from_zero(mxg, cuda_dev, E, dtype):
     half = 0.0 if dtype == "fp32" else torch.finfo(DT[dtype]).eps / 2
     assert np.all(np.abs(_np(dz) - ref) <= G_TOL * size + half * np.abs(ref) + 1e-37)
     assert mxg.device_error() == 0
+
+
+@pytest.mark.filterwarnings("ignore:invalid value")     # the oracle's inf - inf
+@pytest.mark.parametrize("n", [3, 8200])
+@pytest.mark.parametrize("E,groups", [(64, 4), (256, 8)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_infinite_biases_in_groups(mxg, cuda_dev, n, E, groups, score):
+    """A bias of +inf takes its expert always.  In a group whose others are
+    switched off by -inf the sum of the two best has no value and counts as
+    -inf: the best of the other groups are kept, as many as asked for."""
+    inf, per = float("inf"), E // groups
+    z = _logits(n, E, "fp32", 12, cuda_dev)
+    bias = torch.randn(E, device=cuda_dev, generator=torch.Generator(cuda_dev).manual_seed(E)) * 0.05
+    bias[2 * per:3 * per] = -inf
+    bias[2 * per + 1] = inf
+    for kept in (1, 2, groups - 1):
+        _check(mxg, z, 3, score=score, bias=bias, groups=groups, topk_groups=kept, group_score="top2")
+        w, ids = _check(mxg, z, 3, score=score, bias=bias, groups=groups, topk_groups=kept)
+        assert torch.all(ids[:, 0] == 2 * per + 1)
+    bias[2 * per:3 * per] = 0.0
+    bias[2 * per + 1] = bias[5] = inf
+    for how in (dict(), dict(groups=groups, topk_groups=2, group_score="top2"), dict(groups=groups, topk_groups=2)):
+        w, ids = _check(mxg, z, 3, score=score, bias=bias, **how)
+        assert torch.all(ids[:, 0] == 5) and torch.all(ids[:, 1] == 2 * per + 1)
