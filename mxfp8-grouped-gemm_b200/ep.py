@@ -395,6 +395,7 @@ class ExpertParallel:
         self.p2p_max_blocks = p2p_max_blocks
         self.buffers = {}        # name -> PeerBuffer
         self.capacity = {}       # name -> rows
+        self._idle = set()       # receive buffers that every rank has done reading
         self._flag = None
         self._ret_need = None    # rows and row size of the return buffers
         self.marker = None       # optional callable(name): a timing mark on the current stream
@@ -445,7 +446,7 @@ class ExpertParallel:
             dist.barrier(group=self.group)
             for b in self.buffers.values():
                 b.free()
-            self.buffers, self.capacity = {}, {}
+            self.buffers, self.capacity, self._idle = {}, {}, set()
 
     def _barrier(self, device):
         """Stream-ordered rendezvous: returns on the device once every rank's
@@ -453,6 +454,15 @@ class ExpertParallel:
         if self._flag is None or self._flag.device != device:
             self._flag = torch.zeros(1, dtype=torch.int32, device=device)
         dist.all_reduce(self._flag, group=self.group)
+
+    def _claim(self, name, device):
+        """Before rows are stored into the ranks' receive buffers ``name``: a
+        rendezvous, unless a dispatch's (whose counts every rank gathers) came
+        since the last exchange into them.  A rank reads a buffer before its
+        next exchange, so that none is written while another rank reads it."""
+        if name not in self._idle:
+            self._barrier(device)
+        self._idle.discard(name)
 
     def _ensure_buffer(self, name, rows, row_bytes, device):
         """Collective when it (re)allocates: every rank decides from the same
@@ -535,6 +545,7 @@ class ExpertParallel:
         mine = torch.cat([counts, torch.full((1,), n * k, dtype=torch.int32, device=x.device)])
         Cx = torch.empty(W * (E + 1), dtype=torch.int32, device=x.device)
         dist.all_gather_into_tensor(Cx, mine, group=self.group)   # also: every receiver is idle
+        self._idle = {"x", "dy"}
         self._mark("x.counts")
         Cx = Cx.view(W, E + 1)
         Chx = Cx.cpu().numpy().astype(np.int64)
@@ -578,6 +589,7 @@ class ExpertParallel:
         if like or split:
             buf = self.buffers["x"]
             rows, _ = self.capacity["x"]
+            self._claim("x", x.device)
             local = buf.view(m_pad, x)
             self.p2p.zero_pad_rows(local, plan.back_rank)
             self._mark("x.plan")
@@ -625,6 +637,7 @@ class ExpertParallel:
         beside the exchange) instead of one SM kernel storing to the peers."""
         if plan.back_rank is not None and copy_engines:
             m_pad = plan.back_rank.numel()
+            self._claim(buffer, x.device)
             buf = self.buffers[buffer]
             rows, row_bytes = self.capacity[buffer]
             if x.shape[0] and x.element_size() * x[0].numel() != row_bytes:
@@ -646,6 +659,7 @@ class ExpertParallel:
             return local
         if plan.back_rank is not None:
             m_pad = plan.back_rank.numel()
+            self._claim(buffer, x.device)
             buf = self.buffers[buffer]
             rows, row_bytes = self.capacity[buffer]
             if x.shape[0] and x.element_size() * x[0].numel() != row_bytes:
@@ -734,10 +748,13 @@ class ExpertParallel:
     def dispatch_sent(self, rows: torch.Tensor, plan: DispatchPlan, buffer: str = "dy",
                       copy_engines: bool = False) -> torch.Tensor:
         """``dispatch_like`` of rows [n*k, H'] that are in send order already, one
-        for each (token, choice): the gradient that ``combine_grad`` gives."""
+        for each (token, choice): the gradient that ``combine_grad`` gives.
+        Call it (as ``dispatch_like``) on the stream that read the buffer's
+        earlier rows."""
         if plan.back_rank is None:
             recv_buf = self._a2a(rows, plan.recv_rows, plan.recv_splits, plan.send_splits)
             return self.ops.gather(recv_buf, plan.idx, plan.idx.numel())
+        self._claim(buffer, rows.device)
         buf = self.buffers[buffer]
         capacity, row_bytes = self.capacity[buffer]
         if rows.shape[0] and rows.element_size() * rows[0].numel() != row_bytes:
