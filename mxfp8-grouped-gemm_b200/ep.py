@@ -343,6 +343,8 @@ class DispatchPlan:
     back_rank: torch.Tensor | None = None    # [M_pad] home rank of each padded row (-1: padding)
     back_row: torch.Tensor | None = None     # [M_pad] send position on that rank
     ret_order: torch.Tensor | None = None    # [n_recv] real rows grouped by home rank, rotated
+    most_rows: int = 0                       # the most padded rows of a rank (the same on every rank)
+    most_sent: int = 0                       # the most rows that a rank sends (the same on every rank)
     # copy-engine runs (host arrays: src_row, dst_row, rows, dst_rank), each
     # list of runs ordered by destination rank starting with rank me+1
     runs_dispatch: tuple | None = None       # send-order rows of each slot -> the owner's buffer
@@ -455,11 +457,18 @@ class ExpertParallel:
             self._flag = torch.zeros(1, dtype=torch.int32, device=device)
         dist.all_reduce(self._flag, group=self.group)
 
-    def _claim(self, name, device):
+    def _fits(self, name, rows):
+        """Every rank raises, or none: rows is the same on all."""
+        if rows > self.capacity[name][0]:
+            raise ValueError(f"the {name!r} buffers were laid out again, for {self.capacity[name][0]} rows, since this "
+                             f"plan's dispatch, which needs {rows}: rows of several sizes take an ExpertParallel each")
+
+    def _claim(self, name, plan, device):
         """Before rows are stored into the ranks' receive buffers ``name``: a
         rendezvous, unless a dispatch's (whose counts every rank gathers) came
         since the last exchange into them.  A rank reads a buffer before its
         next exchange, so that none is written while another rank reads it."""
+        self._fits(name, plan.most_rows)
         if name not in self._idle:
             self._barrier(device)
         self._idle.discard(name)
@@ -582,14 +591,14 @@ class ExpertParallel:
             C, self.rank, pad, m_pad, recv_rows)
         plan = DispatchPlan(send_rows, slot_pos, None, None, None, None,
                             group_rows, padded[self.rank].tolist(), recv_rows, n, k,
-                            slot_start, dest_base, back_rank, back_row, ret_order)
+                            slot_start, dest_base, back_rank, back_row, ret_order, need, int(sent.max()))
         split = int(split) if 0 < int(split) < El else 0
         like = also_gather is not None and tuple(also_gather.shape) == tuple(x.shape) \
             and also_gather.dtype == x.dtype
         if like or split:
             buf = self.buffers["x"]
             rows, _ = self.capacity["x"]
-            self._claim("x", x.device)
+            self._claim("x", plan, x.device)
             local = buf.view(m_pad, x)
             self.p2p.zero_pad_rows(local, plan.back_rank)
             self._mark("x.plan")
@@ -637,7 +646,7 @@ class ExpertParallel:
         beside the exchange) instead of one SM kernel storing to the peers."""
         if plan.back_rank is not None and copy_engines:
             m_pad = plan.back_rank.numel()
-            self._claim(buffer, x.device)
+            self._claim(buffer, plan, x.device)
             buf = self.buffers[buffer]
             rows, row_bytes = self.capacity[buffer]
             if x.shape[0] and x.element_size() * x[0].numel() != row_bytes:
@@ -659,7 +668,7 @@ class ExpertParallel:
             return local
         if plan.back_rank is not None:
             m_pad = plan.back_rank.numel()
-            self._claim(buffer, x.device)
+            self._claim(buffer, plan, x.device)
             buf = self.buffers[buffer]
             rows, row_bytes = self.capacity[buffer]
             if x.shape[0] and x.element_size() * x[0].numel() != row_bytes:
@@ -698,6 +707,7 @@ class ExpertParallel:
         if plan.back_rank is not None:
             if buffer not in self.buffers:
                 self._ensure_ret(buffer, y_local.device)
+            self._fits(buffer, plan.most_sent)
             buf = self.buffers[buffer]
             rows, row_bytes = self.capacity[buffer]
             if y_local.shape[0] and y_local.element_size() * y_local[0].numel() != row_bytes:
@@ -723,6 +733,7 @@ class ExpertParallel:
             raise ValueError("return_target needs the peer-memory transport")
         if buffer not in self.buffers:
             self._ensure_ret(buffer, like.device)
+        self._fits(buffer, plan.most_sent)
         rows, row_bytes = self.capacity[buffer]
         if like.element_size() * int(np.prod(like.shape[1:])) != row_bytes:
             raise ValueError("result rows must have the dispatched rows' size")
@@ -754,7 +765,7 @@ class ExpertParallel:
         if plan.back_rank is None:
             recv_buf = self._a2a(rows, plan.recv_rows, plan.recv_splits, plan.send_splits)
             return self.ops.gather(recv_buf, plan.idx, plan.idx.numel())
-        self._claim(buffer, rows.device)
+        self._claim(buffer, plan, rows.device)
         buf = self.buffers[buffer]
         capacity, row_bytes = self.capacity[buffer]
         if rows.shape[0] and rows.element_size() * rows[0].numel() != row_bytes:

@@ -169,3 +169,32 @@ def test_two_layers_over_peer_memory(tmp_path, dx):
             assert len(rows) == len(want)
             for i, (a, b) in enumerate(zip(rows, want)):
                 assert np.array_equal(a, b), (r, mode, i)
+
+
+def _laid_out_again(rank):
+    par, said = _parallel(True), []
+    # 164 tokens' 492 rows: 246 at least on one rank; two a rank need 2 * 2 * 3 rows and 4 * 31 of padding, 136
+    big, wide, small = _inputs(rank, [91, 73][rank], 1), _inputs(rank, 4, 2, 2 * H), _inputs(rank, 2, 3)
+    first = _forward(par, *big[:3], False)
+    _forward(par, *wide[:3], False)
+    last = _forward(par, *small[:3], False)
+    dsent, _ = par.combine_grad(big[3], first[2], first[1], big[2])
+    for call in (lambda: par.dispatch_sent(dsent, first[1]), lambda: par.dispatch_like(big[3], first[1]),
+                 lambda: par.combine_send(first[0], first[1]), lambda: par.return_target(first[1], first[0])):
+        try:
+            call()
+            said.append("no error")
+        except ValueError as e:
+            said.append("refused" if "laid out again" in str(e) else str(e))
+    got = _backward(par, last, small[2], small[3], False, True, 0.0)       # the latest plan goes on
+    par.close()
+    ref = _parallel(False)
+    want = _backward(ref, _forward(ref, *small[:3], False), small[2], small[3], False, True, 0.0)
+    return said, all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_plans_of_buffers_laid_out_again_are_refused(tmp_path):
+    """Rows of another size, then a small batch of the first size, leave smaller
+    buffers than the first plan's: every rank refuses it, and nobody waits."""
+    got = _run(_laid_out_again, (), tmp_path)
+    assert got == {r: (["refused"] * 4, True) for r in range(2)}
