@@ -4,10 +4,14 @@ gradients around the expert GEMMs, on one rank, and a training step with AdamW.
 A token with k choices is the same work as k tokens with one choice each, in
 the same send order, so ``step`` on such a batch gives every expected result
 bit for bit."""
+import multiprocessing as mp
+import os
+
 import numpy as np
 import pytest
 import torch
 
+from ep_support import free_port
 from oracle import router_oracle as ro
 
 pytestmark = pytest.mark.gpu
@@ -119,3 +123,66 @@ def test_refusals(mxg, cuda_dev):
     fwd = layer.forward(x, z, mxg.moe.Router(2))
     with pytest.raises(ValueError, match="dout"):
         layer.backward(fwd, d.float())
+
+
+def _two_rank_worker(rank, world, port, q):
+    try:
+        import datetime
+
+        import torch.distributed as dist
+        os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+        torch.cuda.set_device(rank)
+        dist.init_process_group("nccl", rank=rank, world_size=world, timeout=datetime.timedelta(seconds=60))
+        from conftest import load_pkg
+        mxg = load_pkg()
+        dev = torch.device("cuda", rank)
+        E, H, I = 8, 256, 128
+        El = E // world
+        g = torch.Generator(device=dev).manual_seed(9)
+        wgu = (torch.randn(E, 2 * I, H, generator=g, device=dev) * 0.05).to(torch.bfloat16)
+        wd = (torch.randn(E, H, I, generator=g, device=dev) * 0.05).to(torch.bfloat16)
+        mine = slice(rank * El, (rank + 1) * El)
+        router = mxg.moe.Router(2, score="sigmoid")
+        big, small = (_batch(n, E, H, dev, 20 + 2 * i + rank) for i, n in enumerate(([300, 217][rank], [7, 0][rank])))
+        res = {}
+        for dx in (True, False):
+            for name, transport, comm, ce in (("nccl", "nccl", False, False), ("p2p", "p2p", False, False),
+                                              ("p2p_side", "p2p", True, False), ("p2p_ce", "p2p", True, True)):
+                ep = mxg.ExpertParallel(E, transport=transport)
+                a, b = (mxg.moe.ExpertFFN(ep, wgu[mine], wd[mine], compute_dx=dx, copy_engines=ce,
+                                          comm_stream=torch.cuda.Stream() if comm else None) for _ in range(2))
+                got = []
+                for _ in range(2):       # both forwards before both backwards
+                    fa, fb = a.forward(*big[:2], router), b.forward(*small[:2], router)
+                    gb, ga = b.backward(fb, small[2]), a.backward(fa, big[2])
+                    got += [fa.out, fb.out, *ga, *gb]
+                torch.cuda.synchronize()
+                assert mxg.device_error() == 0
+                res[dx, name] = [t.float().cpu().numpy() for t in got if t is not None]
+                ep.close()
+        dist.barrier()
+        dist.destroy_process_group()
+        q.put((rank, res))
+    except Exception:
+        import traceback
+        q.put((rank, traceback.format_exc()))
+
+
+def test_two_layers_over_two_ranks():
+    """Layers of different batches share one ExpertParallel over two GPUs: every
+    exchange gives the bytes of the all-to-all transport."""
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs 2 GPUs")
+    ctx = mp.get_context("spawn")
+    q, port = ctx.Queue(), free_port()
+    procs = [ctx.Process(target=_two_rank_worker, args=(r, 2, port, q)) for r in range(2)]
+    for p in procs:
+        p.start()
+    res = dict(q.get(timeout=600) for _ in procs)
+    for p in procs:
+        p.join(timeout=60)
+    for r in range(2):
+        assert isinstance(res[r], dict), res[r]
+        for (dx, name), got in res[r].items():
+            for i, (a, b) in enumerate(zip(got, res[r][dx, "nccl"])):
+                assert np.array_equal(a, b), (r, dx, name, i)
