@@ -40,7 +40,7 @@ extern "C" {
 
 /* ---- status codes ---------------------------------------------------- */
 #define MXG_OK 0
-#define MXG_ERR_INVALID_ARGUMENT 1    /* null pointer, negative size, bad enum */
+#define MXG_ERR_INVALID_ARGUMENT 1    /* null pointer to data (not of an empty array), negative size, bad enum */
 #define MXG_ERR_BAD_SHAPE 2           /* dims not multiples of 32, too large    */
 #define MXG_ERR_MISALIGNED 3          /* base pointer not 16-byte aligned       */
 #define MXG_ERR_WORKSPACE_TOO_SMALL 4

@@ -1666,7 +1666,7 @@ extern "C" int mxg_grouped_wgrad(const void* go, const void* go_scales, const vo
   int st = check_common(num_groups, m, n, k, out_dtype, offs, offs_len, offs_kind);
   if (st) return st;
   if (m % 32 != 0 || k % 16 != 0) return MXG_ERR_BAD_SHAPE;
-  if (!go || !ia || !out || !workspace) return MXG_ERR_INVALID_ARGUMENT;
+  if (!out || (m > 0 && (!go || !ia || !workspace))) return MXG_ERR_INVALID_ARGUMENT;
   if (!aligned16(go) || !aligned16(ia) || !aligned16(out) || !aligned16(workspace))
     return MXG_ERR_MISALIGNED;
   if (m == 0) {  // no tokens: every dW[e] is zero
@@ -1704,7 +1704,7 @@ extern "C" int mxg_grouped_wgrad_run(const void* go, const void* ia, int num_gro
                         MXG_OFFS_SIZES);
   if (st) return st;
   if (m % 32 != 0 || k % 16 != 0) return MXG_ERR_BAD_SHAPE;
-  if (!go || !ia || !out || !workspace) return MXG_ERR_INVALID_ARGUMENT;
+  if (!out || (m > 0 && (!go || !ia || !workspace))) return MXG_ERR_INVALID_ARGUMENT;
   if (!aligned16(go) || !aligned16(ia) || !aligned16(out) || !aligned16(workspace))
     return MXG_ERR_MISALIGNED;
   if (m == 0) {

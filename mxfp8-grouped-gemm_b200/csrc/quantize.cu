@@ -614,7 +614,7 @@ static int launch_dual(DualArgs a, void* stream, int64_t row0 = 0, int64_t row_e
   a.row0 = row0;
   a.row_end = row_end;
   if ((a.q == nullptr) != (a.s == nullptr) || (a.qt == nullptr) != (a.st == nullptr) ||
-      (a.q == nullptr && a.qt == nullptr))
+      (a.q == nullptr && a.qt == nullptr && a.rows > 0))
     return MXG_ERR_INVALID_ARGUMENT;
   if (a.rows % 32 != 0 || a.cols % 32 != 0) return MXG_ERR_BAD_SHAPE;
   if ((a.q && !aligned16(a.q)) || (a.qt && !aligned16(a.qt))) return MXG_ERR_MISALIGNED;
@@ -655,8 +655,8 @@ using namespace mxg;
 
 extern "C" int mxg_quantize_rowwise(const void* x_bf16, int64_t rows, int64_t cols, void* q_e4m3,
                                     void* scales_e8m0, void* stream) {
-  if (!x_bf16 || !q_e4m3 || !scales_e8m0) return MXG_ERR_INVALID_ARGUMENT;
   if (rows < 0 || cols < 0) return MXG_ERR_INVALID_ARGUMENT;
+  if (rows > 0 && cols > 0 && (!x_bf16 || !q_e4m3 || !scales_e8m0)) return MXG_ERR_INVALID_ARGUMENT;
   if (cols % 32 != 0) return MXG_ERR_BAD_SHAPE;
   if (!aligned16(x_bf16) || !aligned16(q_e4m3)) return MXG_ERR_MISALIGNED;
   if (rows == 0 || cols == 0) return MXG_OK;
@@ -675,8 +675,8 @@ extern "C" int mxg_quantize_rowwise(const void* x_bf16, int64_t rows, int64_t co
 
 extern "C" int mxg_quantize_colwise(const void* x_bf16, int64_t rows, int64_t cols, void* qt_e4m3,
                                     void* scales_t_e8m0, void* stream) {
-  if (!x_bf16 || !qt_e4m3 || !scales_t_e8m0) return MXG_ERR_INVALID_ARGUMENT;
   if (rows < 0 || cols < 0) return MXG_ERR_INVALID_ARGUMENT;
+  if (rows > 0 && cols > 0 && (!x_bf16 || !qt_e4m3 || !scales_t_e8m0)) return MXG_ERR_INVALID_ARGUMENT;
   if (rows % 32 != 0 || cols % 2 != 0) return MXG_ERR_BAD_SHAPE;
   if (!aligned16(x_bf16) || !aligned16(qt_e4m3)) return MXG_ERR_MISALIGNED;
   if (rows == 0 || cols == 0) return MXG_OK;
@@ -697,8 +697,9 @@ extern "C" int mxg_quantize_colwise(const void* x_bf16, int64_t rows, int64_t co
 
 extern "C" int mxg_transpose_u8(const void* src, int64_t rows, int64_t cols, void* dst,
                                 void* stream) {
-  if (!src || !dst || rows < 0 || cols < 0) return MXG_ERR_INVALID_ARGUMENT;
+  if (rows < 0 || cols < 0) return MXG_ERR_INVALID_ARGUMENT;
   if (rows == 0 || cols == 0) return MXG_OK;
+  if (!src || !dst) return MXG_ERR_INVALID_ARGUMENT;
   if ((rows + 63) / 64 > 65535) return MXG_ERR_BAD_SHAPE;
   int st = check_device();
   if (st) return st;
@@ -711,7 +712,7 @@ extern "C" int mxg_transpose_u8(const void* src, int64_t rows, int64_t cols, voi
 extern "C" int mxg_quantize_dual(const void* x_bf16, int64_t rows, int64_t cols, void* q_e4m3,
                                  void* scales_e8m0, void* qt_e4m3, void* scales_t_e8m0,
                                  void* stream) {
-  if (!x_bf16) return MXG_ERR_INVALID_ARGUMENT;
+  if (!x_bf16 && rows > 0) return MXG_ERR_INVALID_ARGUMENT;
   if (!aligned16(x_bf16)) return MXG_ERR_MISALIGNED;
   DualArgs a{reinterpret_cast<const uint4*>(x_bf16), nullptr, rows, cols, 0,
              reinterpret_cast<uint8_t*>(q_e4m3), reinterpret_cast<uint8_t*>(scales_e8m0),
@@ -722,7 +723,7 @@ extern "C" int mxg_quantize_dual(const void* x_bf16, int64_t rows, int64_t cols,
 extern "C" int mxg_quantize_dual_rows(const void* x_bf16, int64_t rows, int64_t cols, int64_t row_begin,
                                       int64_t row_end, void* q_e4m3, void* scales_e8m0, void* qt_e4m3,
                                       void* scales_t_e8m0, void* stream) {
-  if (!x_bf16 || row_end < 0) return MXG_ERR_INVALID_ARGUMENT;
+  if ((!x_bf16 && rows > 0) || row_end < 0) return MXG_ERR_INVALID_ARGUMENT;
   if (!aligned16(x_bf16)) return MXG_ERR_MISALIGNED;
   DualArgs a{reinterpret_cast<const uint4*>(x_bf16), nullptr, rows, cols, 0,
              reinterpret_cast<uint8_t*>(q_e4m3), reinterpret_cast<uint8_t*>(scales_e8m0),
@@ -733,7 +734,7 @@ extern "C" int mxg_quantize_dual_rows(const void* x_bf16, int64_t rows, int64_t 
 extern "C" int mxg_swiglu_quantize(const void* gu_bf16, int64_t rows, int64_t inter, void* q_e4m3,
                                    void* scales_e8m0, void* qt_e4m3, void* scales_t_e8m0,
                                    void* stream) {
-  if (!gu_bf16) return MXG_ERR_INVALID_ARGUMENT;
+  if (!gu_bf16 && rows > 0) return MXG_ERR_INVALID_ARGUMENT;
   if (!aligned16(gu_bf16)) return MXG_ERR_MISALIGNED;
   DualArgs a{reinterpret_cast<const uint4*>(gu_bf16), nullptr, rows, inter, inter,
              reinterpret_cast<uint8_t*>(q_e4m3), reinterpret_cast<uint8_t*>(scales_e8m0),
@@ -744,7 +745,7 @@ extern "C" int mxg_swiglu_quantize(const void* gu_bf16, int64_t rows, int64_t in
 extern "C" int mxg_swiglu_bwd_quantize(const void* gu_bf16, const void* dh_bf16, int64_t rows,
                                        int64_t inter, void* q_e4m3, void* scales_e8m0,
                                        void* qt_e4m3, void* scales_t_e8m0, void* stream) {
-  if (!gu_bf16 || !dh_bf16) return MXG_ERR_INVALID_ARGUMENT;
+  if ((!gu_bf16 || !dh_bf16) && rows > 0) return MXG_ERR_INVALID_ARGUMENT;
   if (!aligned16(gu_bf16) || !aligned16(dh_bf16)) return MXG_ERR_MISALIGNED;
   DualArgs a{reinterpret_cast<const uint4*>(gu_bf16), reinterpret_cast<const uint4*>(dh_bf16),
              rows, 2 * inter, inter, reinterpret_cast<uint8_t*>(q_e4m3),

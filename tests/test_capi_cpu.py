@@ -66,3 +66,22 @@ def test_status_codes_match_header(mxg):
     assert codes, "no status codes found in the header"
     for name, value in codes.items():
         assert getattr(mxg._lib, name) == int(value), name
+
+
+def test_pointers_to_nothing_may_be_null(mxg):
+    """Tensors without elements have no address: zero rows are no error."""
+    L = mxg._lib.load()
+    assert L.mxg_quantize_rowwise(None, 0, 64, None, None, None) == 0
+    assert L.mxg_quantize_colwise(None, 0, 64, None, None, None) == 0
+    assert L.mxg_quantize_dual(None, 0, 64, None, None, None, None, None) == 0
+    assert L.mxg_quantize_dual_rows(None, 0, 64, 0, 0, None, None, None, None, None) == 0
+    assert L.mxg_swiglu_quantize(None, 0, 64, None, None, None, None, None) == 0
+    assert L.mxg_swiglu_bwd_quantize(None, None, 0, 64, None, None, None, None, None) == 0
+    assert L.mxg_transpose_u8(None, 0, 64, None, None) == 0
+    # as before where there is something, and for shapes that no row count allows
+    assert L.mxg_quantize_dual(None, 32, 64, 16, 16, None, None, None) == 1
+    assert L.mxg_quantize_dual(16, 32, 64, None, None, None, None, None) == 1
+    assert L.mxg_swiglu_bwd_quantize(16, None, 32, 64, 16, 16, None, None, None) == 1
+    assert L.mxg_transpose_u8(None, 4, 64, 16, None) == 1
+    assert L.mxg_quantize_dual(None, 0, 48, None, None, None, None, None) == 2
+    assert L.mxg_grouped_wgrad(None, None, 16, None, 16, 2, 2, 2, 64, 64, 64, 16, 0, 16, 1 << 20, None) == 1

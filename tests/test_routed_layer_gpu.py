@@ -186,3 +186,25 @@ def test_two_layers_over_two_ranks():
         for (dx, name), got in res[r].items():
             for i, (a, b) in enumerate(zip(got, res[r][dx, "nccl"])):
                 assert np.array_equal(a, b), (r, dx, name, i)
+
+
+@pytest.mark.parametrize("dx", [True, False])
+def test_no_rows(mxg, cuda_dev, dx):
+    """A rank without tokens whose experts nobody chose (small batches over many
+    ranks): empty outputs, weight gradients of zero."""
+    E, H, I = 8, 128, 64
+    wgu, wd, layer = _layer(mxg, E, H, I, cuda_dev, compute_dx=dx)
+    x, z, d = (t[:0] for t in _batch(4, E, H, cuda_dev))
+    fwd = layer.forward(x, z, mxg.moe.Router(2))
+    got = layer.backward(fwd, d)
+    assert fwd.out.shape == (0, H) and got.dlogits.shape == (0, E) and fwd.weights.shape == (0, 2)
+    assert got.dx is None if not dx else got.dx.shape == (0, H)
+    one = layer.step(x, fwd.ids, fwd.weights, d)
+    for dw, w in ((got.dw_gate_up, wgu), (got.dw_down, wd), (one.dw_gate_up, wgu), (one.dw_down, wd)):
+        assert dw.shape == w.shape and torch.all(dw == 0)
+    assert one.out.shape == (0, H) and mxg.device_error() == 0
+    # the update of such a step: the weights only decay
+    opt = mxg.optim.AdamW([wgu, wd], lr=0.0)
+    keep = wgu.clone()
+    opt.step([got.dw_gate_up, got.dw_down])
+    assert torch.equal(wgu, keep)
