@@ -71,8 +71,9 @@ __device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
 
 // Random bits: 32x32 -> 64-bit products by odd constants, the halves xored,
 // two of them for each of (seed, step), block and element.  Means, spread and
-// correlations of both halves, between neighbours, blocks and steps, are
-// those of independent uniform draws to within sampling error.
+// bits of both halves, and their correlations with one another and between
+// neighbours, blocks, steps and seeds, are those of independent uniform draws
+// to within the sampling error of 2^18 draws (a test).
 constexpr uint32_t kM1 = 0x6A09C55Du, kM2 = 0x5D1B8E63u, kStep = 0x9E2F4D8Bu, kAdd = 0x3C7A15E9u;
 __device__ __forceinline__ uint32_t mix(uint32_t x, uint32_t by) {
   const uint64_t p = uint64_t(x) * by;

@@ -183,3 +183,39 @@ def test_adamw_refuses_settings_beyond_fp32(mxg):
         assert mxg._lib.load().mxg_adamw_step(mxg._lib.adamw_args(
             16, 16, begin.ctypes.data, grads.ctypes.data, kinds.ctypes.data, 16, 16, 0, 0, 0, 16, 16, 0, lr, 0.9,
             0.99, eps, 0, 1, 4096, 32, 0), None) == 1
+
+
+def test_random_words_pass_for_independent_uniform_draws():
+    """Means, spreads and single bits of both words' halves, and correlations
+    between the halves, neighbours, blocks, steps and seeds, over 2^18 draws.
+    A mean of n uniform draws is off by sqrt(1 / 12 n), a mean square by
+    sqrt(4 / 45 n), a bit's by 1 / 2 sqrt(n), a correlation by 1 / sqrt(n): 5.5
+    of each, which one of these 500 figures passes by chance once in 5 * 10^4."""
+    n, off = 1 << 18, 5.5
+
+    def halves(seed, step, first):
+        h, more = ao.words(seed, step, first, n)
+        return [x.astype(np.float64) / 65536 + 2.0 ** -17
+                for w in (h, more) for x in (w >> ao.U(16), w & ao.U(0xFFFF))]
+
+    def apart(x, y):
+        x, y = x - 0.5, y - 0.5
+        assert abs(12 * np.mean(x * y)) <= off / np.sqrt(x.size)
+
+    for seed, step, first in ((0, 1, 0), (1234, 41, 256 * 7), (2 ** 63 + 5, 100_000, 2 ** 33), (1, 2, 0)):
+        here = halves(seed, step, first)
+        for x in here:
+            assert abs(np.mean(x) - 0.5) <= off * np.sqrt(1 / 12 / n)
+            assert abs(np.mean(x * x) - 1 / 3) <= off * np.sqrt(4 / 45 / n)
+            word = (x * 65536).astype(np.int64)
+            for bit in range(16):
+                assert abs(np.mean(word >> bit & 1) - 0.5) <= off / 2 / np.sqrt(n)
+            for gap in (1, 2, 4, 32, 128, 256, 512, 4096):     # neighbours, lanes, blocks, chunks
+                apart(x[:-gap], x[gap:])
+        others = [halves(seed, step + 1, first), halves(seed + 1, step, first), halves(seed ^ 1 << 40, step, first),
+                  halves(seed, step, first + n)]
+        for i, x in enumerate(here):
+            for y in here[i + 1:]:
+                apart(x, y)
+            for other in others:
+                apart(x, other[i])
