@@ -408,6 +408,11 @@ __global__ void __launch_bounds__(kRouterThreads) router_topk_kernel(const __gri
     const float big = a.sigmoid ? sigmoid_fast(top) : inv;
     near = 0x1p-24f * big * (a.sigmoid ? 14.0f + 3.0f * fmaxf(0.0f, -top) : 2.0f * V + 40.0f) + 0x1p-124f;
     again = a.sigmoid && top < -80.0f;                               // the scores vanish in fp32
+    if (a.sigmoid && !a.bias) {
+      // in a group's sum a NaN counts as -inf, a logit of -inf as its score, 0: in the order below they are one
+#pragma unroll
+      for (int v = 0; v < V; ++v) again |= z[v] != z[v];
+    }
   }
   if (a.bias) {
     float b[V];

@@ -573,3 +573,23 @@ def test_infinite_biases_in_groups(mxg, cuda_dev, n, E, groups, score):
     for how in (dict(), dict(groups=groups, topk_groups=2, group_score="top2"), dict(groups=groups, topk_groups=2)):
         w, ids = _check(mxg, z, 3, score=score, bias=bias, **how)
         assert torch.all(ids[:, 0] == 5) and torch.all(ids[:, 1] == 2 * per + 1)
+
+
+@pytest.mark.parametrize("E,groups", [(16, 8), (64, 32), (96, 6), (256, 8)])
+def test_nan_in_sums_of_groups(mxg, cuda_dev, E, groups):
+    """Sigmoid scores without a bias, groups by the sum of their two best: a NaN
+    is ordered as -inf there too, while a logit of -inf has the score 0."""
+    z = _logits(60, E, "fp32", 13, cuda_dev)
+    u = torch.rand(60, E, generator=torch.Generator(cuda_dev).manual_seed(2), device=cuda_dev)
+    z[u < 0.2] = -float("inf")
+    z[20:][u[20:] > 0.8] = float("nan")
+    per = E // groups
+    z[40:, :per] = float("nan")                  # a group whose one expert is far ahead, beside NaN alone
+    z[40:, 0] = 9.0
+    for kept in (1, groups // 2):
+        for k in (1, min(per, 4)):
+            w, ids = mxg.ops.router_topk(z, k, score="sigmoid", groups=groups, topk_groups=kept, group_score="top2")
+            ref = ro.router(_np(z), k, score="sigmoid", groups=groups, topk_groups=kept, group_score="top2")
+            full = np.isfinite(np.take_along_axis(_np(z), ref[1].astype(np.int64), 1)).all(1)
+            assert np.array_equal(ids.cpu().numpy()[full], ref[1][full]) and full[:20].any() and full[20:].any()
+            assert np.all(np.abs(w.cpu().numpy()[full] - ref[0][full]) <= W_TOL * ref[0][full])
