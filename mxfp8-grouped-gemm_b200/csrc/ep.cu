@@ -231,7 +231,9 @@ __global__ void __launch_bounds__(128) combine_kernel(const __nv_bfloat16* __res
 // products are summed in a fixed order: over a thread's columns, over the
 // warp, over the warps.  The first `fill_blocks` blocks write zeros to the
 // rows that no position names: each marks the positions of its kFillRows rows
-// that it finds in the whole table (4 bytes a choice beside 4 * hidden).
+// that it finds in the whole table (4 bytes a choice beside 4 * hidden), then
+// zeroes the others alone, which is meant for few: of 131072 rows of 7168 none
+// 641 us, 1% 675, 10% 1613.
 constexpr int kFillRows = 32768;
 
 __device__ __forceinline__ void zero_unnamed_rows(const int32_t* __restrict__ inv, int64_t n, int64_t first,

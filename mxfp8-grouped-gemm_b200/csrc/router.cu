@@ -677,7 +677,9 @@ __global__ void __launch_bounds__(kRouterThreads) router_rows_kernel(const __gri
   }
 
   // values of 16 below the largest logit, of 2 below the largest s + bias,
-  // share the lowest step: where that is chosen, the slow selection decides
+  // share the lowest step: where that is chosen, or holds the best of a group,
+  // the slow selection decides (16384 x 256 fp32, logits of standard deviation
+  // 1.5, 5 and 10: 8.4, 16.5, 37 us; a group switched off: 117)
   const float scale = BIAS ? 0.5f : 0.0625f, steps = scale * float(1u << (31 - IB));
   const float shift = __fmaf_rd(-largest, scale, 1.0f - 0x1p-22f);  // down: no value reaches 1
   uint32_t key[NC][8];
