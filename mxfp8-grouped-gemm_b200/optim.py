@@ -90,7 +90,7 @@ class AdamW:
             self._copies.append(total if c else -1)
             total += s if c else 0
         dev, n = self.device, max(self.offsets[-1], _lib.ADAMW_BLOCK)
-        with torch.no_grad():
+        with torch.inference_mode(False), torch.no_grad():      # state that any mode may change in place
             self.exp_avg_scale = self.exp_avg_sq_scale = self.master = None
             if state_bits == 8:
                 self.exp_avg = torch.zeros(n, dtype=torch.uint8, device=dev)
@@ -104,9 +104,9 @@ class AdamW:
                 for p, at in zip(params, self._copies):
                     if at >= 0:
                         self.master[at:at + p.numel()].copy_(p.detach().reshape(-1))
-        self._table = torch.empty(len(params) * _ENTRY.itemsize, dtype=torch.uint8, device=dev)
-        self._step = torch.zeros(1, dtype=torch.int64, device=dev)
-        self._done = torch.zeros(1, dtype=torch.int32, device=dev)
+            self._table = torch.empty(len(params) * _ENTRY.itemsize, dtype=torch.uint8, device=dev)
+            self._step = torch.zeros(1, dtype=torch.int64, device=dev)
+            self._done = torch.zeros(1, dtype=torch.int32, device=dev)
         # What a thread block takes at a time: about 128 shares, long runs where there is much.  us of a bf16 step
         # with 32 / 8 bits at 4096, 8192, 32768: 1 M values 6.7 / 8.6, 6.7 / 7.9, 13.8 / 15.7; 64 M 330 / 289,
         # 339 / 219, 337 / 185.

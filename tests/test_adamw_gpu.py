@@ -407,3 +407,23 @@ def test_tensors_without_memory_are_refused(mxg, cuda_dev):
     assert opt.state_dict()["step"] == 0
     opt.step(g)
     assert opt.state_dict()["step"] == 1 and mxg.device_error() == 0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_made_in_inference_mode(mxg, cuda_dev, bits):
+    """The state is changed in place outside that mode too."""
+    a = _make([(300,), (77,)], [BF, F32], 70, cuda_dev)
+    b = [x.clone() for x in a]
+    g = _make([(300,), (77,)], [F32, F32], 71, cuda_dev)
+    one = mxg.optim.AdamW(a, state_bits=bits)
+    with torch.inference_mode():
+        two = mxg.optim.AdamW(b, state_bits=bits)
+        two.step(g)
+    one.step(g)
+    one.weight_decay = two.weight_decay = 0.5
+    one.step(g), two.step(g)
+    two.load_state_dict({k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in one.state_dict().items()})
+    with torch.inference_mode():
+        two.step(g)
+    one.step(g)
+    assert all(torch.equal(x, y) for x, y in zip(a, b)) and torch.equal(one.exp_avg, two.exp_avg)
