@@ -50,8 +50,9 @@ class AdamW:
     at every step.  ``lr``, ``betas``, ``eps`` and ``weight_decay`` may be set
     between steps; a graph captured before keeps its ``betas``, ``eps``, number
     ``lr`` and gradients' addresses, and from the next ``step`` call on takes
-    over a new ``weight_decay`` and the addresses of tensors that have moved.  One optimiser's steps run one after the other: do not
-    issue them on several streams at once."""
+    over a new ``weight_decay`` and the addresses of tensors that have moved.
+    One optimiser's steps run one after the other: do not issue them on several
+    streams at once."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay=0.01, *,
                  state_bits: int = 32, master_weights: bool = True, seed: int = 0):
